@@ -58,7 +58,8 @@ enum {
     SDFOAM_ERR_CUDA = 3         /* a CUDA runtime call failed */
 };
 
-enum { SDFOAM_F32 = 0, SDFOAM_F16 = 1 };
+enum { SDFOAM_F32 = 0, SDFOAM_F16 = 1, SDFOAM_BF16 = 2 };
+enum { SDFOAM_U32 = 0, SDFOAM_I32 = 1, SDFOAM_I64 = 2 };
 enum { SDFOAM_ALPHA_STANDARD = 0, SDFOAM_ALPHA_NEUS = 1 };
 enum { SDFOAM_PINHOLE = 0, SDFOAM_FISHEYE = 1 };
 
@@ -450,6 +451,30 @@ SDFOAM_API int sdfoam_mlp_deactivate(const void *da, int lda, const void *act, i
                                      int cols, void *dz, int ldz, sdfoam_stream_t stream);
 SDFOAM_API int sdfoam_mlp_decode(const float *points, const float *center, uint32_t n, int multires,
                                  const void *denc, int ld, float *dpoints, sdfoam_stream_t stream);
+
+/* Rows of a table at given ids (site attributes or codes at the sites that
+ * sdfoam_nn, sdfoam_farthest_neighbor or a walk returned):
+ *   out[i, :] = scale * table[ids[i], :]
+ * table [rows, columns] of dtype, ld >= columns elements between rows; ids [n]
+ * of id_type; out [n, columns] contiguous, of the table's type.  An id outside
+ * [0, rows) -- the UINT32_MAX that stands for "none", or a negative one --
+ * names no row: its output row is zero.  The product is fp32, rounded once;
+ * with scale 1 the rows are copied bit for bit.  columns <= 2^20. */
+SDFOAM_API int sdfoam_lookup_rows(const void *table, uint32_t rows, uint32_t columns, uint64_t ld, uint32_t dtype,
+                                  const void *ids, uint64_t n, uint32_t id_type, float scale, void *out,
+                                  sdfoam_stream_t stream);
+/* The gradient of sdfoam_lookup_rows with respect to the table:
+ *   grad_table[v, :] = scale * sum over i with ids[i] = v of grad[i, :]
+ * grad [n, columns] of dtype, ld elements between rows; grad_table [rows,
+ * columns] contiguous, of the same type, written completely (zeros where no id
+ * names the row).  The sums are fp32 over a stable sort of the ids, in an
+ * order that depends on n and ids alone: the same bits every run.  n < 2^31.
+ * Workspace: sdfoam_lookup_rows_workspace_bytes, 256-byte aligned. */
+SDFOAM_API size_t sdfoam_lookup_rows_workspace_bytes(uint64_t n, uint32_t rows, uint32_t columns);
+SDFOAM_API int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, uint64_t ld, uint32_t dtype,
+                                           const void *ids, uint64_t n, uint32_t id_type, float scale,
+                                           void *grad_table, uint32_t rows, void *workspace, size_t workspace_bytes,
+                                           sdfoam_stream_t stream);
 
 /* Allocation-free sdfoam_trace_forward.  No counterpart in the reference: it
  * exists for callers that cannot allocate device memory -- hosts reaching this

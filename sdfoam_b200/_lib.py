@@ -15,6 +15,10 @@ LIB_PATH = os.environ.get("SDFOAM_B200_LIB") or os.path.join(HERE, "libsdfoam_b2
 SDFOAM_OK = 0
 SDFOAM_F32 = 0
 SDFOAM_F16 = 1
+SDFOAM_BF16 = 2
+SDFOAM_U32 = 0
+SDFOAM_I32 = 1
+SDFOAM_I64 = 2
 SDFOAM_ALPHA_STANDARD = 0
 SDFOAM_ALPHA_NEUS = 1
 SDFOAM_PINHOLE = 0
@@ -57,6 +61,9 @@ EXPORTED = (
     "sdfoam_mlp_activate",
     "sdfoam_mlp_deactivate",
     "sdfoam_mlp_decode",
+    "sdfoam_lookup_rows",
+    "sdfoam_lookup_rows_workspace_bytes",
+    "sdfoam_lookup_rows_backward",
 )
 
 
@@ -238,6 +245,13 @@ def load():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = args
+    u64 = ctypes.c_uint64
+    lib.sdfoam_lookup_rows.restype = ctypes.c_int
+    lib.sdfoam_lookup_rows.argtypes = [vp, u32, u32, u64, u32, vp, u64, u32, f32, vp, vp]
+    lib.sdfoam_lookup_rows_workspace_bytes.restype = ctypes.c_size_t
+    lib.sdfoam_lookup_rows_workspace_bytes.argtypes = [u64, u32, u32]
+    lib.sdfoam_lookup_rows_backward.restype = ctypes.c_int
+    lib.sdfoam_lookup_rows_backward.argtypes = [vp, u32, u64, u32, vp, u64, u32, f32, vp, u32, vp, ctypes.c_size_t, vp]
     _lib = lib
     return lib
 

@@ -42,6 +42,23 @@ int check_foam(const sdfoam_foam *foam) {
     return SDFOAM_OK;
 }
 
+// sdfoam_lookup_rows and its gradient.
+int check_lookup(uint32_t dtype, uint32_t id_type, uint32_t columns, uint64_t ld) {
+    if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported table type");
+    if (id_type > SDFOAM_I64) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported id type");
+    if (columns > (1u << 20)) return fail(SDFOAM_ERR_INVALID, "a table has at most 2^20 columns");
+    if (ld < columns || (ld >> 40)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
+    return SDFOAM_OK;
+}
+
+bool aligned_to(const void *p, uint32_t dtype) {
+    return (reinterpret_cast<uintptr_t>(p) & (dtype == SDFOAM_F32 ? 3u : 1u)) == 0;
+}
+
+bool aligned_ids(const void *p, uint32_t id_type) {
+    return (reinterpret_cast<uintptr_t>(p) & (id_type == SDFOAM_I64 ? 7u : 3u)) == 0;
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // [R,4] attribute-typed rows: 16 bytes (float32) or 8 bytes (float16) each.
@@ -594,6 +611,47 @@ int sdfoam_mlp_decode(const float *points, const float *center, uint32_t n, int 
     cudaError_t e =
         launch_mlp_decode(points, center, n, multires, denc, ld, dpoints, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_mlp_decode");
+}
+
+int sdfoam_lookup_rows(const void *table, uint32_t rows, uint32_t columns, uint64_t ld, uint32_t dtype,
+                       const void *ids, uint64_t n, uint32_t id_type, float scale, void *out,
+                       sdfoam_stream_t stream) {
+    int rc = check_lookup(dtype, id_type, columns, ld);
+    if (rc != SDFOAM_OK) return rc;
+    if (n > 0 && columns > 0 && (!ids || !out || (rows > 0 && !table)))
+        return fail(SDFOAM_ERR_INVALID, "table, ids and out must be non-NULL");
+    if (n >> 40) return fail(SDFOAM_ERR_INVALID, "too many ids");
+    if (!aligned_to(table, dtype) || !aligned_to(out, dtype) || !aligned_ids(ids, id_type))
+        return fail(SDFOAM_ERR_INVALID, "table, ids and out must be aligned to their elements");
+    cudaError_t e = launch_lookup_rows(table, rows, columns, ld, dtype, ids, n, id_type, scale, out,
+                                       reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_lookup_rows");
+}
+
+size_t sdfoam_lookup_rows_workspace_bytes(uint64_t n, uint32_t rows, uint32_t columns) {
+    return n >> 31 ? 0 : lookup_grad_workspace_bytes(static_cast<uint32_t>(n), rows, columns);
+}
+
+int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, uint64_t ld, uint32_t dtype, const void *ids,
+                                uint64_t n, uint32_t id_type, float scale, void *grad_table, uint32_t rows,
+                                void *workspace, size_t workspace_bytes, sdfoam_stream_t stream) {
+    int rc = check_lookup(dtype, id_type, columns, ld);
+    if (rc != SDFOAM_OK) return rc;
+    if (n >> 31) return fail(SDFOAM_ERR_INVALID, "the gradient takes fewer than 2^31 ids");
+    if (rows > 0 && columns > 0 && (!grad_table || (n > 0 && (!grad || !ids))))
+        return fail(SDFOAM_ERR_INVALID, "grad, ids and grad_table must be non-NULL");
+    if (!aligned_to(grad, dtype) || !aligned_to(grad_table, dtype) || !aligned_ids(ids, id_type))
+        return fail(SDFOAM_ERR_INVALID, "grad, ids and grad_table must be aligned to their elements");
+    const size_t need = sdfoam_lookup_rows_workspace_bytes(n, rows, columns);
+    if (rows > 0 && columns > 0 && need > 0) {
+        if (!workspace || workspace_bytes < need) return fail(SDFOAM_ERR_INVALID, "workspace is too small");
+        if (reinterpret_cast<uintptr_t>(workspace) & 255u)
+            return fail(SDFOAM_ERR_INVALID, "workspace must be 256-byte aligned");
+    }
+    cudaError_t e = launch_lookup_rows_backward(grad, ld, columns, dtype, ids, static_cast<uint32_t>(n), id_type,
+                                                scale, grad_table, rows, workspace,
+                                                reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_lookup_rows_backward");
 }
 
 const char *sdfoam_last_error(void) { return g_last_error.c_str(); }

@@ -79,13 +79,23 @@ struct SortLayout {
 };
 SortLayout sort_layout(uint32_t n);
 
-// Stable LSD radix sort of n (key, value) pairs by the whole 32-bit key: four
-// 8-bit passes over one unit.  keys[cur] / vals[cur] hold the input; on return
+// Stable LSD radix sort of n (key, value) pairs by the low `bits` bits of the
+// 32-bit key (the others zero): 8-bit passes over one unit.  keys[cur] / vals[cur] hold the input; on return
 // cur names the pair of buffers holding the result.  hist holds
 // radix_hist_entries(n) words, totals 256.
 size_t radix_hist_entries(uint32_t n);
 cudaError_t launch_radix_sort_pairs(uint32_t *const keys[2], uint32_t *const vals[2], uint32_t n, uint32_t *hist,
-                                    uint32_t *totals, int &cur, cudaStream_t stream);
+                                    uint32_t *totals, int &cur, cudaStream_t stream, int bits = 32);
+
+// Table rows at given ids and the table's gradient (rows.cu).  dtype, itype:
+// SDFOAM_F32 / F16 / BF16, SDFOAM_I32 (also unsigned) / I64; ld in elements.
+size_t lookup_grad_workspace_bytes(uint32_t n, uint32_t rows, uint32_t columns);
+cudaError_t launch_lookup_rows(const void *table, uint32_t rows, uint32_t columns, size_t ld, uint32_t dtype,
+                               const void *ids, uint64_t n, uint32_t itype, float scale, void *out,
+                               cudaStream_t stream);
+cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t columns, uint32_t dtype, const void *ids,
+                                        uint32_t n, uint32_t itype, float scale, void *out, uint32_t rows,
+                                        void *workspace, cudaStream_t stream);
 
 // Gradient workspace layout:
 //   attr_acc   float4 [N * V]   per-site attribute gradient rows
