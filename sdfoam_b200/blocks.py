@@ -1,0 +1,267 @@
+"""Products in 8 bits: e4m3 values with one scale per block of 128.
+
+The sdfnet's layers multiply bf16 matrices; these operators do the same
+contractions on e4m3 operands at twice the tensor cores' rate and half the
+bytes, for networks over sites whose width or number makes that worth the
+precision (e4m3 keeps four significant bits).
+
+``quantize_blocks`` turns a matrix into e4m3 values and power-of-two scales,
+``dequantize_blocks`` turns them back, ``block_matmul`` multiplies two such
+matrices (with any fp32 scales, as a checkpoint may bring them), and
+``block_linear`` is a layer for training: its forward and both of its
+gradients are 8-bit products of operands quantized on the way.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.SDFOAM_F32, torch.float16: _lib.SDFOAM_F16, torch.bfloat16: _lib.SDFOAM_BF16}
+_E4M3 = torch.float8_e4m3fn
+_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return (n + _BLOCK - 1) // _BLOCK
+
+
+def _cuda(what: str, x: torch.Tensor, device=None):
+    if x.device.type != "cuda":
+        raise RuntimeError(f"{what} must be on CUDA device")
+    if device is not None and x.device != device:
+        raise RuntimeError(f"{what} must be on the device of the other arguments")
+
+
+def _matrix(x: torch.Tensor) -> torch.Tensor:
+    """x itself when its rows are contiguous (any distance apart), else a copy."""
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+# One word per device in pinned host memory, which a kernel that gives up
+# waiting writes and the host reads without a copy.
+_flags: dict = {}
+
+
+def _flag(device: torch.device) -> torch.Tensor:
+    f = _flags.get(device.index)
+    if f is None:
+        f = _flags[device.index] = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    elif f[0]:
+        _raise(f)
+    return f
+
+
+def _raise(f):
+    f.zero_()
+    raise RuntimeError("an 8-bit product gave up waiting on the tensor-core pipeline and wrote NaN")
+
+
+def check_block_flags():
+    """Waits for the devices that have run 8-bit products and raises
+    RuntimeError if one of them gave up waiting on the tensor-core pipeline
+    (the next product on the device raises it too)."""
+    for index, f in _flags.items():
+        torch.cuda.synchronize(index)
+        if f[0]:
+            _raise(f)
+
+
+def _values(rows: int, columns: int, device) -> torch.Tensor:
+    """An e4m3 matrix whose rows start on 16 bytes."""
+    ld = (columns + 15) // 16 * 16
+    v = torch.empty((rows, ld), dtype=_E4M3, device=device)
+    return v if ld == columns else v[:, :columns]
+
+
+def _quantize(x, block_rows, normal, turned):
+    """(values, scales) or None of x and of x turned."""
+    x = _matrix(x)
+    m, k = x.shape
+    dev = x.device
+    v = s = vt = st = None
+    if normal:
+        v = _values(m, k, dev)
+        s = torch.empty((m if block_rows == 1 else _blocks(m), _blocks(k)), dtype=torch.float32, device=dev)
+    if turned:
+        vt = _values(k, m, dev)
+        st = torch.empty((k if block_rows == 1 else _blocks(k), _blocks(m)), dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        _lib.check(lib.sdfoam_block_quantize(
+            x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, k, block_rows,
+            v.data_ptr() if normal else None, max(v.stride(0), k) if normal else 0, s.data_ptr() if normal else None,
+            vt.data_ptr() if turned else None, max(vt.stride(0), m) if turned else 0,
+            st.data_ptr() if turned else None, torch.cuda.current_stream().cuda_stream))
+    return (v, s) if normal else None, (vt, st) if turned else None
+
+
+def quantize_blocks(x: torch.Tensor, block_rows: int = 1, transpose: bool = False):
+    """(values, scales) of a matrix in blocks of ``block_rows`` x 128 (1:
+    activations, 128: weights), of ``x.t()`` with ``transpose``.
+
+    values: float8_e4m3fn, rows 16 bytes aligned; scales: float32
+    [ceil(rows / block_rows), ceil(columns / 128)], per block the smallest
+    power of two s >= 2^-126 with ``448 s`` at least the block's largest
+    magnitude (1 for a block of zeros).  values = x / s to the nearest, ties to
+    even.  Infinities and NaN become NaN and do not count in the block's
+    largest magnitude."""
+    if x.dim() != 2:
+        raise RuntimeError("x must have 2 dimensions")
+    if x.dtype not in _DTYPES:
+        raise RuntimeError("x must have float32, float16 or bfloat16 dtype")
+    if block_rows not in (1, _BLOCK):
+        raise RuntimeError("block_rows must be 1 or 128")
+    _cuda("x", x)
+    return _quantize(x.detach(), block_rows, not transpose, bool(transpose))[int(bool(transpose))]
+
+
+def _block_rows(what: str, values: torch.Tensor, scales: torch.Tensor) -> int:
+    if values.dim() != 2 or scales.dim() != 2:
+        raise RuntimeError(f"{what} and its scales must have 2 dimensions")
+    if values.dtype != _E4M3:
+        raise RuntimeError(f"{what} must have float8_e4m3fn dtype")
+    if scales.dtype != torch.float32:
+        raise RuntimeError(f"the scales of {what} must have float32 dtype")
+    m, k = values.shape
+    if tuple(scales.shape) == (m, _blocks(k)):
+        return 1
+    if tuple(scales.shape) == (_blocks(m), _blocks(k)):
+        return _BLOCK
+    raise RuntimeError(f"the scales of {what} must have shape [{m} or {_blocks(m)}, {_blocks(k)}]")
+
+
+def dequantize_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """values * scales as a contiguous matrix of ``dtype``; the blocks follow
+    from the shape of the scales."""
+    block_rows = _block_rows("values", values, scales)
+    if dtype not in _DTYPES:
+        raise RuntimeError("dtype must be float32, float16 or bfloat16")
+    _cuda("values", values)
+    _cuda("scales", scales, values.device)
+    v, s = _matrix(values), scales.contiguous()
+    m, k = v.shape
+    out = torch.empty((m, k), dtype=dtype, device=v.device)
+    lib = _lib.load()
+    with torch.cuda.device(v.device):
+        _lib.check(lib.sdfoam_block_dequantize(v.data_ptr(), max(v.stride(0), k), s.data_ptr(), block_rows, m, k,
+                                               _DTYPES[dtype], out.data_ptr(),
+                                               torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def _operand(v: torch.Tensor) -> torch.Tensor:
+    """Rows 16 bytes aligned, as the copies into shared memory need them."""
+    m, k = v.shape
+    if v.stride(1) == 1 and v.stride(0) >= k and v.stride(0) % 16 == 0 and v.data_ptr() % 16 == 0:
+        return v
+    out = _values(m, k, v.device)
+    out.copy_(v)
+    return out
+
+
+def _product(a, a_scales, a_rows, b, b_scales, b_rows, bias, out_dtype):
+    a, b = _operand(a), _operand(b)
+    a_scales, b_scales = a_scales.contiguous(), b_scales.contiguous()
+    m, k = a.shape
+    n = b.shape[0]
+    dev = a.device
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    lib = _lib.load()
+    nbytes = lib.sdfoam_block_matmul_workspace_bytes(m, n, k)
+    with torch.cuda.device(dev):
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.check(lib.sdfoam_block_matmul(
+            a.data_ptr(), max(a.stride(0), k), a_scales.data_ptr(), a_rows, m, b.data_ptr(), max(b.stride(0), k),
+            b_scales.data_ptr(), b_rows, n, k, None if bias is None else bias.data_ptr(),
+            0 if bias is None else _DTYPES[bias.dtype], out.data_ptr(), max(n, 1), _DTYPES[out_dtype],
+            None if ws is None else ws.data_ptr(), nbytes, _flag(dev).data_ptr(),
+            torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def _check_bias(bias, n, device):
+    if bias is not None:
+        if bias.dtype not in _DTYPES or tuple(bias.shape) != (n,):
+            raise RuntimeError(f"bias must be a float32, float16 or bfloat16 vector of {n}")
+        _cuda("bias", bias, device)
+
+
+def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+                 bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(a * a_scales) @ (b * b_scales).t() + bias`` of e4m3 matrices a [M, K]
+    and b [N, K] with a scale per 1 x 128 or 128 x 128 block (any fp32 values;
+    the shape of the scales says which).  fp32 sums in a fixed order, rounded
+    once to ``out_dtype`` (float32, float16 or bfloat16).  Not differentiable;
+    see :func:`block_linear`."""
+    a_rows = _block_rows("a", a, a_scales)
+    b_rows = _block_rows("b", b, b_scales)
+    if a.shape[1] != b.shape[1]:
+        raise RuntimeError(f"a and b must have the same number of columns, got {a.shape[1]} and {b.shape[1]}")
+    if out_dtype not in _DTYPES:
+        raise RuntimeError("out_dtype must be float32, float16 or bfloat16")
+    _cuda("a", a)
+    for what, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
+        _cuda(what, t, a.device)
+    _check_bias(bias, b.shape[0], a.device)
+    bias = None if bias is None else bias.detach().contiguous()
+    return _product(a, a_scales.detach(), a_rows, b, b_scales.detach(), b_rows, bias, out_dtype)
+
+
+class _BlockLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        # one pass over each operand writes it in rows and, for the gradient
+        # that reduces along the other axis, turned
+        q, qt = _quantize(x, 1, True, need_w)
+        w, wt = _quantize(weight, _BLOCK, True, need_x)
+        ctx.save_for_backward(*(qt or (None, None)), *(wt or (None, None)))
+        ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        return _product(*q, 1, *w, _BLOCK, None if bias is None else bias.contiguous(), x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        qt, qts, wt, wts = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dx = dw = db = None
+        if need_x or need_w:
+            g, gt = _quantize(grad, 1, need_x, need_w)
+            if need_x:
+                dx = _product(*g, 1, wt, wts, _BLOCK, None, ctx.dtypes[0])
+            if need_w:
+                dw = _product(*gt, 1, qt, qts, 1, None, ctx.dtypes[1])
+        if need_b:
+            db = grad.sum(0, dtype=torch.float32).to(ctx.dtypes[2])
+        return dx, dw, db
+
+
+def block_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.t() + bias`` with 8-bit products: x [..., K], weight [N, K]
+    (float32, float16 or bfloat16), output of x's type.
+
+    With Q the values that :func:`quantize_blocks` keeps, in blocks of 1 x 128
+    of x and 128 x 128 of the weight:
+
+        y = Q(x) Q(weight)^T + bias
+        dx = Q(dy) Q(weight),  dweight = Q(dy^T) Q(x^T)^T,  dbias = sum dy
+
+    the blocks of dy along the reduction of each product (its columns for dx,
+    its rows for dweight).  For a weight that stays as it is, quantize it once
+    and call :func:`block_matmul`."""
+    if weight.dim() != 2 or x.dim() < 1:
+        raise RuntimeError("weight must have 2 dimensions and x at least 1")
+    if x.shape[-1] != weight.shape[1]:
+        raise RuntimeError(f"x must have {weight.shape[1]} columns, got {x.shape[-1]}")
+    for what, t in (("x", x), ("weight", weight)):
+        if t.dtype not in _DTYPES:
+            raise RuntimeError(f"{what} must have float32, float16 or bfloat16 dtype")
+    _cuda("x", x)
+    _cuda("weight", weight, x.device)
+    _check_bias(bias, weight.shape[0], x.device)
+    rows = 1
+    for d in x.shape[:-1]:
+        rows *= d
+    y = _BlockLinear.apply(x.reshape(rows, x.shape[-1]), weight, bias)
+    return y.reshape(*x.shape[:-1], weight.shape[0])

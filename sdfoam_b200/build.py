@@ -19,13 +19,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsdfoam_b200.so")
-SOURCES = ["cells.cu", "trace.cu", "aabb.cu", "foam_ops.cu", "sort.cu", "delaunay.cu", "tets.cu", "mlp.cu", "mlp_tc.cu", "rows.cu", "capi.cu", "noalloc.cu"]
-HEADERS = ["foam_device.cuh", "foam_internal.h", "voronoi_cell.cuh"]
+SOURCES = ["cells.cu", "trace.cu", "aabb.cu", "foam_ops.cu", "sort.cu", "delaunay.cu", "tets.cu", "mlp.cu", "mlp_tc.cu", "rows.cu", "block_quant.cu", "block_mm.cu",
+           "capi.cu", "noalloc.cu"]
+HEADERS = ["foam_device.cuh", "foam_internal.h", "tcgen05.cuh", "voronoi_cell.cuh"]
 # The walk, spatial and Delaunay kernels share their floating-point contract
 # with the CPU restatement, so they are built with -fmad=false (only written
 # fmaf() calls fuse).  The sdfnet MLP stages produce bf16 activations checked
 # by tolerance and may contract multiply-adds.
-CONTRACTED = {"mlp.cu", "mlp_tc.cu"}
+CONTRACTED = {"mlp.cu", "mlp_tc.cu", "block_mm.cu"}
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [

@@ -42,6 +42,14 @@ int check_foam(const sdfoam_foam *foam) {
     return SDFOAM_OK;
 }
 
+// A matrix of e4m3 blocks (also: the tiles of an output).
+int check_blocks(uint64_t m, uint64_t k, int block_rows) {
+    if (block_rows != 1 && block_rows != 128) return fail(SDFOAM_ERR_INVALID, "block_rows must be 1 or 128");
+    if ((m >> 31) || (k >> 31) || (((m + 127) / 128) * ((k + 127) / 128)) >> 31)
+        return fail(SDFOAM_ERR_INVALID, "matrix too large: 2^31 rows, columns or blocks of 128 x 128");
+    return SDFOAM_OK;
+}
+
 // sdfoam_lookup_rows and its gradient.
 int check_lookup(uint32_t dtype, uint32_t id_type, uint32_t columns, uint64_t ld) {
     if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported table type");
@@ -652,6 +660,73 @@ int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, uint64_t ld,
                                                 scale, grad_table, rows, workspace,
                                                 reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_lookup_rows_backward");
+}
+
+int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m, uint64_t k, int block_rows,
+                          void *values, uint64_t ldv, float *scales, void *turned, uint64_t ldt,
+                          float *turned_scales, sdfoam_stream_t stream) {
+    int rc = check_blocks(m, k, block_rows);
+    if (rc != SDFOAM_OK) return rc;
+    if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
+    if (ld < k || (ld >> 40)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
+    if (m > 0 && k > 0) {
+        if (!x || (!values && !turned) || (values && !scales) || (turned && !turned_scales))
+            return fail(SDFOAM_ERR_INVALID, "x and values with scales (or turned with turned_scales) must be non-NULL");
+        if (!aligned_to(x, dtype)) return fail(SDFOAM_ERR_INVALID, "x must be aligned to its elements");
+        if ((values && (ldv % 16 || ldv < k || !aligned16(values))) || (turned && (ldt % 16 || ldt < m || !aligned16(turned))))
+            return fail(SDFOAM_ERR_INVALID, "rows of values must be multiples of 16 bytes and 16-byte aligned");
+    }
+    cudaError_t e = launch_block_quantize(x, ld, dtype, static_cast<uint32_t>(m), static_cast<uint32_t>(k), block_rows,
+                                          values, ldv, scales, turned, ldt, turned_scales,
+                                          reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_quantize");
+}
+
+int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, int block_rows, uint64_t m,
+                            uint64_t k, uint32_t dtype, void *out, sdfoam_stream_t stream) {
+    int rc = check_blocks(m, k, block_rows);
+    if (rc != SDFOAM_OK) return rc;
+    if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
+    if (m > 0 && k > 0 && (!values || !scales || !out))
+        return fail(SDFOAM_ERR_INVALID, "values, scales and out must be non-NULL");
+    if (ldv < k || (ldv >> 40)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
+    if (!aligned_to(out, dtype)) return fail(SDFOAM_ERR_INVALID, "out must be aligned to its elements");
+    cudaError_t e = launch_block_dequantize(values, ldv, scales, block_rows, static_cast<uint32_t>(m),
+                                            static_cast<uint32_t>(k), dtype, out, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_dequantize");
+}
+
+size_t sdfoam_block_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_t k) {
+    if ((m >> 31) || (n >> 31) || (k >> 31)) return 0;
+    return block_matmul_workspace_bytes(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(k));
+}
+
+int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint64_t m,
+                        const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint64_t n, uint64_t k,
+                        const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo, uint32_t out_dtype,
+                        void *workspace, size_t workspace_bytes, int *error, sdfoam_stream_t stream) {
+    int rc = check_blocks(m, k, a_block_rows);
+    if (rc == SDFOAM_OK) rc = check_blocks(n, k, b_block_rows);
+    if (rc == SDFOAM_OK) rc = check_blocks(m, n, 1);
+    if (rc != SDFOAM_OK) return rc;
+    if (out_dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported output type");
+    if (bias && bias_dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported bias type");
+    if (m == 0 || n == 0) return SDFOAM_OK;
+    if (!out || (k > 0 && (!a || !b || !a_scales || !b_scales || !error)))
+        return fail(SDFOAM_ERR_INVALID, "a, b, their scales, out and error must be non-NULL");
+    if (k > 0 && (lda % 16 || ldb % 16 || lda < k || ldb < k || (lda >> 40) || (ldb >> 40) || !aligned16(a) || !aligned16(b)))
+        return fail(SDFOAM_ERR_INVALID, "rows of a and b must be multiples of 16 bytes and 16-byte aligned");
+    if (ldo < n || (ldo >> 38)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
+    if (!aligned_to(out, out_dtype) || (bias && !aligned_to(bias, bias_dtype)))
+        return fail(SDFOAM_ERR_INVALID, "out and bias must be aligned to their elements");
+    const size_t need = sdfoam_block_matmul_workspace_bytes(m, n, k);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(SDFOAM_ERR_INVALID, "workspace is too small or not 16-byte aligned");
+    cudaError_t e = launch_block_matmul(a, lda, a_scales, a_block_rows, static_cast<uint32_t>(m), b, ldb, b_scales,
+                                        b_block_rows, static_cast<uint32_t>(n), static_cast<uint32_t>(k), bias,
+                                        bias_dtype, out, ldo, out_dtype, workspace, error,
+                                        reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_matmul");
 }
 
 const char *sdfoam_last_error(void) { return g_last_error.c_str(); }

@@ -97,6 +97,19 @@ cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t co
                                         uint32_t n, uint32_t itype, float scale, void *out, uint32_t rows,
                                         void *workspace, cudaStream_t stream);
 
+// e4m3 with a scale per block of 1 x 128 or 128 x 128 (block_quant.cu), and
+// the product of two such matrices (block_mm.cu).
+cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint32_t m, uint32_t k, int block_rows,
+                                  void *values, size_t ldv, float *scales, void *turned, size_t ldt,
+                                  float *turned_scales, cudaStream_t stream);
+cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, int block_rows, uint32_t m,
+                                    uint32_t k, uint32_t dtype, void *out, cudaStream_t stream);
+size_t block_matmul_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
+cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint32_t m,
+                                const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint32_t n,
+                                uint32_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
+                                uint32_t out_dtype, void *workspace, int *error, cudaStream_t stream);
+
 // Gradient workspace layout:
 //   attr_acc   float4 [N * V]   per-site attribute gradient rows
 //   point_acc  float4 [N]       per-site position gradient (x, y, z, 0)

@@ -31,6 +31,7 @@
 #include <cuda_bf16.h>
 
 #include "foam_internal.h"
+#include "tcgen05.cuh"
 
 namespace sdfoam_b200 {
 
@@ -49,8 +50,6 @@ constexpr uint32_t kBoxBytes = 32 * 64;  // an epilogue warp's output box: 32 ro
 constexpr uint32_t kSmemBytes = kWBytes + kStages * kABytes + kEpiWarps * kBoxBytes + (2 * kTileN + 8) * 4 + 1024 + 256;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr uint32_t kMaxPolls = 1u << 26;
-constexpr uint64_t kWaitNs = 500000000ull;  // half a second: a tile's wait is microseconds
 constexpr float kBeta = 100.0f;
 constexpr float kInvBeta = 0.01f;
 
@@ -58,74 +57,6 @@ constexpr float kInvBeta = 0.01f;
 // bf16 (bits 7-9, 10-12 = 1), both K-major, N >> 3 at bit 17, M >> 4 at 24.
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTileN >> 3) << 17) |
                             (uint32_t(kTileM >> 4) << 24);
-
-// Shared-memory matrix descriptor of a K-major tile written by TMA with the
-// 128-byte swizzle: start address >> 4, leading offset 1 (unused for this
-// layout), stride 1024 bytes between 8-row groups, version 1, layout 2.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr) {
-    uint64_t d = uint64_t((smem_addr >> 4) & 0x3fffu);
-    d |= uint64_t(1) << 16;
-    d |= uint64_t(1024 >> 4) << 32;
-    d |= uint64_t(1) << 46;
-    d |= uint64_t(2) << 61;
-    return d;
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Polls the phase of the given parity.  False when *abort is raised or after
-// kWaitNs nanoseconds (which raises *abort); abort == nullptr: only the time
-// bound (the clean-up waits).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
-    const uint64_t t0 = global_ns();
-    for (uint32_t i = 0; i < kMaxPolls; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n"
-            "}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 255u) == 255u) {
-            if (abort && *abort) return false;
-            if (global_ns() - t0 > kWaitNs) break;
-        }
-    }
-    if (abort) *abort = 1;
-    return false;
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 
 __device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
     asm volatile(
@@ -146,10 +77,6 @@ __device__ __forceinline__ void mma_bf16_id(uint32_t tmem_d, uint64_t adesc, uin
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
         "}\n" ::"r"(tmem_d),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v) {
@@ -895,18 +822,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) wgrad_kernel(const __grid_const
         asm volatile("tcgen05.fence::after_thread_sync;");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
     }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
-    return fn;
 }
 
 // 2-D bf16 map of a row-major [rows, cols] matrix with row stride ld
