@@ -478,36 +478,40 @@ SDFOAM_API int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, u
 
 /* e4m3 values with one scale per block of 128, for products in 8 bits.
  *   quantize: x [m, k] of dtype (ld elements between rows) in blocks of
- *     block_rows x 128 (block_rows 1 or 128).  scales[i, j] is the smallest
+ *     block_rows x 128 (block_rows 1 or 128).  A block's scale is the smallest
  *     power of two s >= 2^-126 with 448 s >= the block's largest magnitude (1
  *     for a block of zeros), values[r, c] = x[r, c] / scale rounded to the
  *     nearest e4m3, ties to even.  Infinities and NaN do not count in the
  *     largest magnitude and become NaN.  values [m, ldv] and scales
- *     [ceil(m / block_rows), ceil(k / 128)] (NULL: not written); turned
- *     [k, ldt] and turned_scales [ceil(k / block_rows), ceil(m / 128)] are the
- *     same of x^T, its blocks along x's rows (NULL: not written).  ldv and ldt
+ *     [ceil(k / 128), ceil(m / block_rows)], the rows' scales of one block of
+ *     columns after another (NULL: not written); turned [k, ldt] and
+ *     turned_scales [ceil(m / 128), ceil(k / block_rows)] are the same of x^T,
+ *     its blocks along x's rows (NULL: not written).  ldv and ldt
  *     are multiples of 16 of at least k and m, values and turned 16-byte
  *     aligned; columns up to the next multiple of 16 are written as zeros.
- *   dequantize: out [m, k] contiguous of dtype = values * scales.
+ *   dequantize: out [m, k] contiguous of dtype = values * scales, the scale of
+ *     row block i and column block j at scales[i * scale_row + j * scale_block].
  * m and k below 2^31; ceil(m / 128) * ceil(k / 128) below 2^31. */
 SDFOAM_API int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m, uint64_t k,
                                      int block_rows, void *values, uint64_t ldv, float *scales, void *turned,
                                      uint64_t ldt, float *turned_scales, sdfoam_stream_t stream);
-SDFOAM_API int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, int block_rows,
-                                       uint64_t m, uint64_t k, uint32_t dtype, void *out, sdfoam_stream_t stream);
+SDFOAM_API int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, uint64_t scale_row,
+                                       uint64_t scale_block, int block_rows, uint64_t m, uint64_t k, uint32_t dtype,
+                                       void *out, sdfoam_stream_t stream);
 /* The product of two such matrices on the tcgen05 tensor cores:
  *   out[m, n] = sum_j a_scales[m, j] b_scales[n, j] sum_(k in block j) a[m, k] b[n, k] + bias[n]
  * a [m, k] and b [n, k] e4m3, lda and ldb bytes between rows (multiples of 16,
- * 16-byte aligned); scales any fp32 values, one row per block_rows (1 or 128)
- * rows, contiguous [.., ceil(k / 128)].  Sums are fp32 in a fixed order; bias
+ * 16-byte aligned); scales any fp32 values, one per block_rows (1 or 128) rows
+ * and 128 columns, addressed as in sdfoam_block_dequantize.  Sums are fp32 in a fixed order; bias
  * (NULL: none) of bias_dtype; out of out_dtype with ldo elements between rows.
  * *error (device-accessible int) is set to 1 if a tile gave up waiting for its
  * copies or MMAs (its outputs are NaN).  Workspace:
  * sdfoam_block_matmul_workspace_bytes (0: none), 16-byte aligned. */
 SDFOAM_API size_t sdfoam_block_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_t k);
-SDFOAM_API int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint64_t m,
-                                   const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint64_t n,
-                                   uint64_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
+SDFOAM_API int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
+                                   uint64_t a_scale_block, int a_block_rows, uint64_t m, const void *b, uint64_t ldb,
+                                   const float *b_scales, uint64_t b_scale_row, uint64_t b_scale_block,
+                                   int b_block_rows, uint64_t n, uint64_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
                                    uint32_t out_dtype, void *workspace, size_t workspace_bytes, int *error,
                                    sdfoam_stream_t stream);
 

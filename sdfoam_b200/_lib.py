@@ -259,12 +259,12 @@ def load():
     lib.sdfoam_block_quantize.restype = ctypes.c_int
     lib.sdfoam_block_quantize.argtypes = [vp, u64, u32, u64, u64, i32, vp, u64, vp, vp, u64, vp, vp]
     lib.sdfoam_block_dequantize.restype = ctypes.c_int
-    lib.sdfoam_block_dequantize.argtypes = [vp, u64, vp, i32, u64, u64, u32, vp, vp]
+    lib.sdfoam_block_dequantize.argtypes = [vp, u64, vp, u64, u64, i32, u64, u64, u32, vp, vp]
     lib.sdfoam_block_matmul_workspace_bytes.restype = ctypes.c_size_t
     lib.sdfoam_block_matmul_workspace_bytes.argtypes = [u64, u64, u64]
     lib.sdfoam_block_matmul.restype = ctypes.c_int
-    lib.sdfoam_block_matmul.argtypes = [vp, u64, vp, i32, u64, vp, u64, vp, i32, u64, u64, vp, u32, vp, u64, u32, vp,
-                                        ctypes.c_size_t, vp, vp]
+    lib.sdfoam_block_matmul.argtypes = [vp, u64, vp, u64, u64, i32, u64, vp, u64, vp, u64, u64, i32, u64, u64, vp, u32,
+                                        vp, u64, u32, vp, ctypes.c_size_t, vp, vp]
     _lib = lib
     return lib
 

@@ -82,10 +82,10 @@ def _quantize(x, block_rows, normal, turned):
     v = s = vt = st = None
     if normal:
         v = _values(m, k, dev)
-        s = torch.empty((m if block_rows == 1 else _blocks(m), _blocks(k)), dtype=torch.float32, device=dev)
+        s = torch.empty((_blocks(k), m if block_rows == 1 else _blocks(m)), dtype=torch.float32, device=dev).t()
     if turned:
         vt = _values(k, m, dev)
-        st = torch.empty((k if block_rows == 1 else _blocks(k), _blocks(m)), dtype=torch.float32, device=dev)
+        st = torch.empty((_blocks(m), k if block_rows == 1 else _blocks(k)), dtype=torch.float32, device=dev).t()
     lib = _lib.load()
     with torch.cuda.device(dev):
         _lib.check(lib.sdfoam_block_quantize(
@@ -101,7 +101,8 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1, transpose: bool = Fals
     activations, 128: weights), of ``x.t()`` with ``transpose``.
 
     values: float8_e4m3fn, rows 16 bytes aligned; scales: float32
-    [ceil(rows / block_rows), ceil(columns / 128)], per block the smallest
+    [ceil(rows / block_rows), ceil(columns / 128)] with the rows' scales of one
+    block of columns next to each other in memory, per block the smallest
     power of two s >= 2^-126 with ``448 s`` at least the block's largest
     magnitude (1 for a block of zeros).  values = x / s to the nearest, ties to
     even.  Infinities and NaN become NaN and do not count in the block's
@@ -139,13 +140,13 @@ def dequantize_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.d
         raise RuntimeError("dtype must be float32, float16 or bfloat16")
     _cuda("values", values)
     _cuda("scales", scales, values.device)
-    v, s = _matrix(values), scales.contiguous()
+    v, s = _matrix(values), scales
     m, k = v.shape
     out = torch.empty((m, k), dtype=dtype, device=v.device)
     lib = _lib.load()
     with torch.cuda.device(v.device):
-        _lib.check(lib.sdfoam_block_dequantize(v.data_ptr(), max(v.stride(0), k), s.data_ptr(), block_rows, m, k,
-                                               _DTYPES[dtype], out.data_ptr(),
+        _lib.check(lib.sdfoam_block_dequantize(v.data_ptr(), max(v.stride(0), k), s.data_ptr(), s.stride(0), s.stride(1),
+                                               block_rows, m, k, _DTYPES[dtype], out.data_ptr(),
                                                torch.cuda.current_stream().cuda_stream))
     return out
 
@@ -162,7 +163,6 @@ def _operand(v: torch.Tensor) -> torch.Tensor:
 
 def _product(a, a_scales, a_rows, b, b_scales, b_rows, bias, out_dtype):
     a, b = _operand(a), _operand(b)
-    a_scales, b_scales = a_scales.contiguous(), b_scales.contiguous()
     m, k = a.shape
     n = b.shape[0]
     dev = a.device
@@ -172,8 +172,9 @@ def _product(a, a_scales, a_rows, b, b_scales, b_rows, bias, out_dtype):
     with torch.cuda.device(dev):
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         _lib.check(lib.sdfoam_block_matmul(
-            a.data_ptr(), max(a.stride(0), k), a_scales.data_ptr(), a_rows, m, b.data_ptr(), max(b.stride(0), k),
-            b_scales.data_ptr(), b_rows, n, k, None if bias is None else bias.data_ptr(),
+            a.data_ptr(), max(a.stride(0), k), a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), a_rows, m,
+            b.data_ptr(), max(b.stride(0), k), b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), b_rows,
+            n, k, None if bias is None else bias.data_ptr(),
             0 if bias is None else _DTYPES[bias.dtype], out.data_ptr(), max(n, 1), _DTYPES[out_dtype],
             None if ws is None else ws.data_ptr(), nbytes, _flag(dev).data_ptr(),
             torch.cuda.current_stream().cuda_stream))

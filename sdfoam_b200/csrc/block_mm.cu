@@ -14,9 +14,13 @@
 //   * warp 1 (one lane) issues four MMAs (K 32 each) per block into the next
 //     of the TMEM accumulators, releasing ring stages and finished
 //     accumulators with tcgen05.commit;
-//   * warps 2-9 read the accumulators back (warp w: TMEM lanes 32 (w % 4)
+//   * warps 2 and 3 bring the blocks' scales of the tile's rows of P and of Q
+//     into a ring of their own (cp.async), several blocks ahead;
+//   * warps 4-11 read the accumulators back (warp w: TMEM lanes 32 (w % 4)
 //     .., half of the TN columns; one row per thread) and multiply-add them
-//     into registers while the tensor cores fill the next accumulator.
+//     into registers while the tensor cores fill the next accumulator.  Their
+//     sums and two chunks of loads take the registers that the first four
+//     warps give up.
 //
 // The operand with the rows on the TMEM lanes is P, the other Q.  Q is b
 // unless a has few rows (a single token to 64): then a's rows are the narrow
@@ -41,86 +45,156 @@ namespace {
 
 constexpr int kSms = 148;
 constexpr int kTileP = 128;
-constexpr int kBlockK = 128;  // bytes of a row per stage: one swizzle span, one block of scales
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kThreads = 32 * (4 + kEpiWarps);
+// Registers: launched with 168 each (384 threads), the first four warps keep
+// 56 and the others grow to 224: 128 x 56 + 256 x 224 = 384 x 168.
+constexpr int kControlRegs = 56, kEpiRegs = 224;
+constexpr int kBlockK = 128;  // bytes of a row per stage: one swizzle span, one block of scales
 constexpr uint32_t kPBytes = kTileP * kBlockK;  // 16 KB
-constexpr uint32_t kBoxBytes = 32 * 64;         // an epilogue warp's output box: 32 rows of 64 bytes
 constexpr int kSwizzleTiles = 16;               // tiles of P that are walked together (L2)
 
-// TN columns of Q per tile: ring stages that fit, TMEM accumulators.
-template <int TN>
+// TN columns of Q per tile, shared by the CTAs of a pair: ring stages that
+// fit, TMEM accumulators, the epilogue's staging.
+template <int TN, bool PAIR>
 struct Shape {
-    static constexpr uint32_t kQBytes = TN * kBlockK;
-    static constexpr uint32_t kStageBytes = kPBytes + kQBytes;
-    static constexpr int kStages = TN == 256 ? 4 : TN == 128 ? 6 : 8;
+    static constexpr int kCtas = PAIR ? 2 : 1;
+    static constexpr uint32_t kQBytes = TN / kCtas * kBlockK;
+    static constexpr uint32_t kStageBytes = kPBytes + kQBytes;  // per CTA
+    static constexpr int kStages = TN == 256 ? (PAIR ? 4 : 3) : TN == 128 ? 5 : TN == 64 ? 7 : 8;
     static constexpr int kAccs = TN == 256 ? 2 : 4;
     static constexpr uint32_t kTmemCols = uint32_t(TN) * kAccs;
-    static constexpr int kHalf = TN / 2;  // columns of an epilogue warp
-    static constexpr uint32_t kSmem = kStages * kStageBytes + kEpiWarps * kBoxBytes + 2 * TN * 4 + 256 + 1024;
+    static constexpr int kGroups = 2, kCols = TN / kGroups;  // groups of four epilogue warps, their columns
+    // per epilogue warp: its 32 rows x kCols columns of 16 bits, at least a box of 32 x 128 bytes
+    static constexpr uint32_t kBoxBytes = kCols < 32 ? 0 : kCols == 128 ? 8192 : 4096;
+    static constexpr int kScaleStages = 6;
+    static constexpr uint32_t kScaleFloats = kTileP + TN;  // of a block: P's rows, Q's rows
+    static constexpr uint32_t kSmem =
+        kStages * kStageBytes + kEpiWarps * kBoxBytes + (kScaleStages * kScaleFloats + TN) * 4 + 512 + 1024;
+};
+
+// How a tile's rows reach out.
+enum : int {
+    kStoreRows,  // element by element, consecutive lanes on consecutive columns
+    kStoreBox,   // TMA boxes of 32 rows x 128 bytes: rows of out are 16-byte aligned
+    kStoreSpan,  // one tile covers whole contiguous rows: 32 rows are one bulk copy
 };
 
 struct BlockParams {
     uint32_t p_rows, q_rows;
     uint32_t tiles_p, tiles_q;
     uint32_t k_blocks, splits, units;
-    const float *p_scales, *q_scales;  // [ceil(rows >> shift), k_blocks]
+    const float *p_scales, *q_scales;  // of row r and block j: scales[(r >> shift) * row + j * block]
     int p_shift, q_shift;              // 0 or 7: rows per scale as a power of two
+    uint64_t p_scale_row, p_scale_block, q_scale_row, q_scale_block;
     const void *bias;                  // over b's rows (n), or null
     uint32_t bias_dtype;
     void *out;                         // [m, n]
     uint64_t ldo;
     uint32_t out_dtype;
-    int box_store;                     // rows of out allow TMA stores
+    int store;
     float4 *parts;                     // splits > 1: sums of the slices
     int *error;
 };
 
 // tcgen05 instruction descriptor, kind::f8f6f4: D fp32 (bits 4-5 = 1), A and
 // B e4m3 (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
-template <int TN>
+template <int N, bool PAIR>
 __device__ __forceinline__ constexpr uint32_t idesc() {
-    return (1u << 4) | (uint32_t(TN >> 3) << 17) | (uint32_t(kTileP >> 4) << 24);
+    return (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t((PAIR ? 2 * kTileP : kTileP) >> 4) << 24);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t id,
                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(id), "r"(accumulate));
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(id), "r"(accumulate));
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(id), "r"(accumulate));
 }
 
-// 16 (or 8) consecutive columns of the warp's 32 lanes; the values may be
-// used after tmem_wait, which names them so that no use moves before it.
-__device__ __forceinline__ void tmem_load(uint32_t (&r)[16], uint32_t addr) {
+// An arrival at the barrier of both CTAs of the pair (the same place in
+// their shared memory), or of the one CTA, when the MMAs so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit_to_all(uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                bar),
+            "h"(uint16_t(3))
+            : "memory");
+    else
+        mma_commit(bar);
+}
+
+// A pair's copies complete on the first CTA's barrier (bit 24 of a shared
+// address is the rank in the pair).
+template <bool PAIR>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+            "%3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar & 0xfeffffffu)
+            : "memory");
+    else
+        tma_load_2d(dst, map, x, y, bar);
+}
+
+// An arrival at the first CTA's barrier.  Relaxed: what it orders are reads of
+// TMEM, which the tcgen05 fence before it covers; a release at cluster scope
+// waits for every other access too (8192^3: 1084 us with it, 524 without).
+template <bool PAIR>
+__device__ __forceinline__ void arrive_at_first(uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n"
+            ".reg .b32 a;\n"
+            "mapa.shared::cluster.u32 a, %0, 0;\n"
+            "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n"
+            "}\n" ::"r"(bar)
+            : "memory");
+    else
+        mbar_arrive(bar);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// Consecutive columns of the warp's 32 lanes; the values may be used after
+// tmem_wait, which names them so that no use moves before it.
+__device__ __forceinline__ void tmem_load(uint32_t (&r)[8], uint32_t addr) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_load(uint32_t (&r)[8], uint32_t addr) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr));
-}
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-                 :
-                 : "memory");
+    asm volatile(
+        "tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+        :
+        : "memory");
 }
 
 // Two fp32 lanes in one instruction.
@@ -183,72 +257,177 @@ __device__ __forceinline__ Unit unit_of(const BlockParams &P, uint32_t u) {
     return r;
 }
 
-// One 64-byte row per lane (32 rows) of the output through the warp's box:
-// TMA where the rows of out are 16-byte aligned, else whole rows of the box
-// by consecutive lanes.
-__device__ __forceinline__ void store_box(const BlockParams &P, const CUtensorMap *map, unsigned char *box,
-                                          const uint32_t (&w)[16], uint32_t row0, uint32_t col0, uint32_t lane) {
-    const uint32_t sw = (lane >> 1) & 3u;
-    if (P.box_store && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    __syncwarp();
+// Stores a warp's 32 rows x kCols columns (lane = row), at least 32 columns.
+// `stage` is the warp's staging buffer, `row_stage` that of the warps of its
+// rows.  Rows go to shared memory in pieces of 16 bytes, swizzled as the TMA
+// unit (or the element-wise reader) expects: piece q of row r of a box of 128
+// bytes at q ^ (r & 7), of 64 bytes at q ^ ((r / 2) & 3).
+template <int kCols, int kGroups>
+__device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorMap *map, unsigned char *stage,
+                                           unsigned char *row_stage, const uint64_t (&acc)[kCols / 2], uint32_t row0,
+                                           uint32_t col0, uint32_t lane, uint32_t group, uint32_t quarter) {
+    // this warp's previous stores have read the buffer
+    if (P.store != kStoreRows && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    if (P.store == kStoreSpan) {
+        // 16-bit rows of q_rows columns one after another, all groups
+        asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
+        const uint32_t n = P.q_rows;
+        uint16_t *dst = reinterpret_cast<uint16_t *>(row_stage) + lane * n + col0;
 #pragma unroll
-    for (uint32_t q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4 *>(box + lane * 64u + ((q ^ sw) << 4)) =
-            make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-    if (P.box_store) {
+        for (int i = 0; i < kCols / 2; ++i) {
+            const float2 x = unpair(acc[i]);
+            const uint32_t w = pack2(P.out_dtype, x.x, x.y);
+            if (col0 + 2 * i + 1 < n && (n & 1u) == 0) {
+                *reinterpret_cast<uint32_t *>(dst + 2 * i) = w;
+            } else {
+                if (col0 + 2 * i < n) dst[2 * i] = uint16_t(w);
+                if (col0 + 2 * i + 1 < n) dst[2 * i + 1] = uint16_t(w >> 16);
+            }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                             reinterpret_cast<uint64_t>(map)),
-                         "r"(int(col0)), "r"(int(row0)), "r"(smem_u32(box))
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
+        if (group == 0 && row0 < P.p_rows) {
+            const uint32_t bytes = min(32u, P.p_rows - row0) * n * 2, whole = bytes & ~15u;
+            unsigned char *to = static_cast<unsigned char *>(P.out) + uint64_t(row0) * n * 2;
+            if (lane == 0 && whole) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to),
+                             "r"(smem_u32(row_stage)), "r"(whole)
+                             : "memory");
+            }
+            if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            if (lane < (bytes - whole) / 2)
+                reinterpret_cast<uint16_t *>(to + whole)[lane] = reinterpret_cast<uint16_t *>(row_stage + whole)[lane];
         }
         return;
     }
     __syncwarp();
-    if (P.out_dtype == SDFOAM_F32) {
-        const uint32_t c = lane & 15u;
-#pragma unroll 4
-        for (uint32_t r = lane >> 4; r < 32; r += 2) {
-            const uint32_t v = *reinterpret_cast<const uint32_t *>(box + r * 64u + (((c >> 2) ^ ((r >> 1) & 3u)) << 4) + (c & 3u) * 4u);
-            if (row0 + r < P.p_rows && col0 + c < P.q_rows)
-                static_cast<uint32_t *>(P.out)[uint64_t(row0 + r) * P.ldo + col0 + c] = v;
+    const bool wide = P.out_dtype == SDFOAM_F32;
+    constexpr int kCols16 = kCols >= 64 ? 64 : 32;  // columns of a box of 16-bit elements
+    constexpr int kBoxes16 = kCols / kCols16, kBoxes32 = kCols / 32, kFit32 = kBoxes32 >= 2 ? kBoxes32 / 2 : 1;
+    const uint32_t sw16 = kCols16 == 64 ? (lane & 7u) : ((lane >> 1) & 3u);
+    if (!wide) {
+#pragma unroll
+        for (int b = 0; b < kBoxes16; ++b) {
+            unsigned char *box = stage + b * (32 * kCols16 * 2) + lane * (kCols16 * 2);
+#pragma unroll
+            for (int q = 0; q < kCols16 / 8; ++q) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = unpair(acc[(b * kCols16 + q * 8) / 2 + e]);
+                    w[e] = pack2(P.out_dtype, x.x, x.y);
+                }
+                *reinterpret_cast<uint4 *>(box + ((q ^ sw16) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
-    } else {
-#pragma unroll 4
-        for (uint32_t r = 0; r < 32; ++r) {
-            const uint16_t v = *reinterpret_cast<const uint16_t *>(box + r * 64u + (((lane >> 3) ^ ((r >> 1) & 3u)) << 4) + (lane & 7u) * 2u);
-            if (row0 + r < P.p_rows && col0 + lane < P.q_rows)
-                static_cast<uint16_t *>(P.out)[uint64_t(row0 + r) * P.ldo + col0 + lane] = v;
+        if (P.store == kStoreBox) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+                for (int b = 0; b < kBoxes16; ++b)
+                    if (col0 + b * kCols16 < P.q_rows && row0 < P.p_rows)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                         reinterpret_cast<uint64_t>(map)),
+                                     "r"(int(col0 + b * kCols16)), "r"(int(row0)),
+                                     "r"(smem_u32(stage + b * (32 * kCols16 * 2)))
+                                     : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            return;
+        }
+        __syncwarp();
+        for (uint32_t r = 0; r < 32 && row0 + r < P.p_rows; ++r) {
+            const uint32_t sw = kCols16 == 64 ? (r & 7u) : ((r >> 1) & 3u);
+            uint16_t *dst = static_cast<uint16_t *>(P.out) + uint64_t(row0 + r) * P.ldo;
+#pragma unroll
+            for (int j = 0; j < kCols / 32; ++j) {
+                const uint32_t c = j * 32 + lane, b = c / kCols16, in = c % kCols16;
+                const uint16_t v = *reinterpret_cast<const uint16_t *>(
+                    stage + b * (32 * kCols16 * 2) + r * (kCols16 * 2) + (((in >> 3) ^ sw) << 4) + (in & 7u) * 2u);
+                if (col0 + c < P.q_rows) dst[col0 + c] = v;
+            }
+        }
+        __syncwarp();
+        return;
+    }
+    // fp32: boxes of 32 columns, kFit32 of them at a time
+#pragma unroll
+    for (int b0 = 0; b0 < kBoxes32; b0 += kFit32) {
+        if (b0 > 0) {
+            if (P.store == kStoreBox && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+        }
+#pragma unroll
+        for (int b = b0; b < b0 + kFit32; ++b) {
+            unsigned char *box = stage + (b - b0) * 4096 + lane * 128;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float2 x = unpair(acc[b * 16 + q * 2]), y = unpair(acc[b * 16 + q * 2 + 1]);
+                *reinterpret_cast<float4 *>(box + ((q ^ (lane & 7u)) << 4)) = make_float4(x.x, x.y, y.x, y.y);
+            }
+        }
+        if (P.store == kStoreBox) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+                for (int b = b0; b < b0 + kFit32; ++b)
+                    if (col0 + b * 32 < P.q_rows && row0 < P.p_rows)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                         reinterpret_cast<uint64_t>(map)),
+                                     "r"(int(col0 + b * 32)), "r"(int(row0)), "r"(smem_u32(stage + (b - b0) * 4096))
+                                     : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        } else {
+            __syncwarp();
+            for (uint32_t r = 0; r < 32 && row0 + r < P.p_rows; ++r) {
+                float *dst = static_cast<float *>(P.out) + uint64_t(row0 + r) * P.ldo;
+#pragma unroll
+                for (int b = b0; b < b0 + kFit32; ++b) {
+                    const float v = *reinterpret_cast<const float *>(stage + (b - b0) * 4096 + r * 128 +
+                                                                     (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u);
+                    if (col0 + b * 32 + lane < P.q_rows) dst[col0 + b * 32 + lane] = v;
+                }
+            }
+            __syncwarp();
         }
     }
 }
 
 // QROWS: a scale per row of Q (per column of the tile) instead of one per 128.
 // SWAP: P is b and Q is a; the tile is stored turned.
-template <int TN, bool QROWS, bool SWAP>
+// PAIR: two CTAs share a tile of 256 rows of P; each brings its 128 rows and
+// half of the tile's rows of Q, and the first one issues the MMAs
+// (cta_group::2) over both CTAs' shared memory, so that each operand byte
+// brought in feeds twice the work.
+template <int TN, bool QROWS, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                const __grid_constant__ CUtensorMap map_q,
                                                                const __grid_constant__ CUtensorMap map_out,
                                                                const BlockParams P) {
-    using S = Shape<TN>;
-    constexpr int kHalf = S::kHalf;
-    constexpr int kChunk = kHalf < 16 ? kHalf : 16;
+    using S = Shape<TN, PAIR>;
+    constexpr int kCols = S::kCols;
+    constexpr int kChunk = 8;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char *boxes = smem + S::kStages * S::kStageBytes;
-    float *q_scale = reinterpret_cast<float *>(boxes + kEpiWarps * kBoxBytes);  // [2][TN]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(q_scale + 2 * TN);
-    // bars: full[stages], empty[stages], acc_full[accs], acc_empty[accs], drain
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 2 * S::kAccs + 1);
+    float *scales = reinterpret_cast<float *>(boxes + kEpiWarps * S::kBoxBytes);  // [kScaleStages][kTileP + TN]
+    float *bias_s = scales + S::kScaleStages * S::kScaleFloats;                    // [TN]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(bias_s + TN);
+    // bars: full[stages], empty[stages], acc_full[accs], acc_empty[accs],
+    // scale_full[scale stages], scale_empty[scale stages], drain
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::kStages + 2 * S::kAccs + 2 * S::kScaleStages + 1);
     __shared__ volatile int abort_flag;
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const uint32_t first_unit = PAIR ? blockIdx.x / 2 : blockIdx.x, unit_step = PAIR ? gridDim.x / 2 : gridDim.x;
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages;
     const uint32_t acc_full = empty + 8 * S::kStages, acc_empty = acc_full + 8 * S::kAccs;
-    const uint32_t drain = acc_empty + 8 * S::kAccs;
+    const uint32_t scale_full = acc_empty + 8 * S::kAccs, scale_empty = scale_full + 8 * S::kScaleStages;
+    const uint32_t drain = scale_empty + 8 * S::kScaleStages;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -257,190 +436,228 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
         }
         for (int b = 0; b < S::kAccs; ++b) {
             mbar_init(acc_full + 8 * b, 1);
-            mbar_init(acc_empty + 8 * b, kEpiWarps);
+            mbar_init(acc_empty + 8 * b, kEpiWarps * S::kCtas);
+        }
+        for (int s = 0; s < S::kScaleStages; ++s) {
+            mbar_init(scale_full + 8 * s, 64);
+            mbar_init(scale_empty + 8 * s, kEpiWarps);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         abort_flag = 0;
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(S::kTmemCols));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"(S::kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "r"(S::kTmemCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;");
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        // ---- producer ----
-        uint32_t issued = 0;
-        bool ok = true;
-        for (uint32_t u = blockIdx.x; u < P.units && ok; u += gridDim.x) {
-            const Unit t = unit_of(P, u);
-            for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++issued) {
-                const uint32_t s = issued % S::kStages, use = issued / S::kStages;
-                if (use > 0 && !mbar_wait(empty + 8 * s, (use - 1) & 1, &abort_flag)) {
-                    ok = false;
-                    break;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+        if (warp == 0 && lane == 0) {
+            // ---- producer ----
+            uint32_t issued = 0;
+            bool ok = true;
+            for (uint32_t u = first_unit; u < P.units && ok; u += unit_step) {
+                const Unit t = unit_of(P, u);
+                const int p0 = int((t.tp * S::kCtas + rank) * kTileP), q0 = int(t.tq * TN + rank * (TN / S::kCtas));
+                for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++issued) {
+                    const uint32_t s = issued % S::kStages, use = issued / S::kStages;
+                    if (use > 0 && !mbar_wait(empty + 8 * s, (use - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = smem_u32(smem + s * S::kStageBytes);
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, S::kCtas * S::kStageBytes);
+                    load_tile<PAIR>(dst, &map_p, int(kb * kBlockK), p0, full + 8 * s);
+                    load_tile<PAIR>(dst + kPBytes, &map_q, int(kb * kBlockK), q0, full + 8 * s);
                 }
-                unsigned char *dst = smem + s * S::kStageBytes;
-                mbar_expect_tx(full + 8 * s, S::kStageBytes);
-                tma_load_2d(smem_u32(dst), &map_p, int(kb * kBlockK), int(t.tp * kTileP), full + 8 * s);
-                tma_load_2d(smem_u32(dst + kPBytes), &map_q, int(kb * kBlockK), int(t.tq * TN), full + 8 * s);
             }
-        }
-        // own copies: the last use of every stage
-        for (uint32_t l = issued > uint32_t(S::kStages) ? issued - S::kStages : 0; l < issued; ++l)
-            mbar_wait(full + 8 * (l % S::kStages), (l / S::kStages) & 1, nullptr);
-    } else if (warp == 1 && lane == 0) {
-        // ---- MMA issuer: one accumulator per block of 128 ----
-        uint32_t done = 0;
-        bool ok = true;
-        for (uint32_t u = blockIdx.x; u < P.units && ok; u += gridDim.x) {
-            const Unit t = unit_of(P, u);
-            for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++done) {
-                const uint32_t s = done % S::kStages, use = done / S::kStages;
-                const uint32_t b = done % S::kAccs, turn = done / S::kAccs;
-                if ((turn > 0 && !mbar_wait(acc_empty + 8 * b, (turn - 1) & 1, &abort_flag)) ||
-                    !mbar_wait(full + 8 * s, use & 1, &abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;");
-                const uint32_t base = smem_u32(smem + s * S::kStageBytes);
-                const uint64_t ad = sw128_desc(base), bd = sw128_desc(base + kPBytes);
+            // the pair's copies, and the MMAs' releases of the stages, which
+            // arrive here: the last use of every stage
+            for (uint32_t l = issued > uint32_t(S::kStages) ? issued - S::kStages : 0; l < issued; ++l) {
+                if (rank == 0) mbar_wait(full + 8 * (l % S::kStages), (l / S::kStages) & 1, nullptr);
+                if (ok) mbar_wait(empty + 8 * (l % S::kStages), (l / S::kStages) & 1, &abort_flag);
+            }
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            // ---- MMA issuer: one accumulator per block of 128 ----
+            uint32_t done = 0;
+            bool ok = true;
+            for (uint32_t u = first_unit; u < P.units && ok; u += unit_step) {
+                const Unit t = unit_of(P, u);
+                for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++done) {
+                    const uint32_t s = done % S::kStages, use = done / S::kStages;
+                    const uint32_t b = done % S::kAccs, turn = done / S::kAccs;
+                    if ((turn > 0 && !mbar_wait(acc_empty + 8 * b, (turn - 1) & 1, &abort_flag)) ||
+                        !mbar_wait(full + 8 * s, use & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t base = smem_u32(smem + s * S::kStageBytes);
+                    const uint64_t ad = sw128_desc(base), bd = sw128_desc(base + kPBytes);
 #pragma unroll
-                for (int k = 0; k < kBlockK / 32; ++k)
-                    mma_e4m3(tmem + b * TN, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc<TN>(), k > 0 ? 1u : 0u);
-                mma_commit(empty + 8 * s);
-                mma_commit(acc_full + 8 * b);
+                    for (int k = 0; k < kBlockK / 32; ++k)
+                        mma_e4m3<PAIR>(tmem + b * TN, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc<TN, PAIR>(),
+                                       k > 0 ? 1u : 0u);
+                    commit_to_all<PAIR>(acc_full + 8 * b);
+                    commit_to_all<PAIR>(empty + 8 * s);
+                }
             }
+            // no MMA may still be running when the accumulators are freed
+            if constexpr (PAIR)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain) : "memory");
+            else
+                mma_commit(drain);
+            mbar_wait(drain, 0, nullptr);
+        } else if (warp >= 2) {
+            // ---- scales: warp 2 P's, warp 3 Q's (one per row, or one for the
+            // 128 rows that a group of epilogue warps has) ----
+            const uint64_t step = warp == 2 ? P.p_scale_block : P.q_scale_block;
+            const uint32_t to = smem_u32(scales + (warp == 2 ? 0 : kTileP) + lane);
+            uint32_t done = 0;
+            bool ok = true;
+            for (uint32_t u = first_unit; u < P.units && ok; u += unit_step) {
+                const Unit t = unit_of(P, u);
+                constexpr int kQPer = QROWS ? (TN + 31) / 32 : 1, kPer = kQPer > 4 ? kQPer : 4;
+                const float *src[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const uint32_t at = i * 32 + lane;
+                    src[i] = nullptr;
+                    if (warp == 2 && i < 4) {
+                        const uint32_t row = min((t.tp * S::kCtas + rank) * kTileP + at, P.p_rows - 1);
+                        src[i] = P.p_scales + (row >> P.p_shift) * P.p_scale_row + t.k0 * P.p_scale_block;
+                    } else if (warp == 3 && i < kQPer && at < uint32_t(QROWS ? TN : S::kGroups)) {
+                        const uint32_t row = min(t.tq * TN + (QROWS ? at : at * kCols), P.q_rows - 1);
+                        src[i] = P.q_scales + (row >> P.q_shift) * P.q_scale_row + t.k0 * P.q_scale_block;
+                    }
+                }
+                for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++done) {
+                    const uint32_t s = done % S::kScaleStages, use = done / S::kScaleStages;
+                    if (use > 0 && !mbar_wait(scale_empty + 8 * s, (use - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        if (src[i]) {
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + (s * S::kScaleFloats + i * 32) * 4),
+                                         "l"(src[i])
+                                         : "memory");
+                            src[i] += step;
+                        }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(scale_full + 8 * s) : "memory");
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        // no MMA may still be running when the accumulators are freed
-        mma_commit(drain);
-        mbar_wait(drain, 0, nullptr);
-    } else if (warp >= 2) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         // ---- sums and stores; every warp takes every block, also after a
         // wait gave up (the barriers below stay matched) ----
-        const uint32_t quarter = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
-        unsigned char *box = boxes + (warp - 2) * kBoxBytes;
-        uint32_t done = 0;
+        const uint32_t quarter = warp & 3, group = (warp - 4) / 4, et = threadIdx.x - 128;
+        // the warps of a quarter have their staging next to each other
+        unsigned char *row_stage = boxes + quarter * S::kGroups * S::kBoxBytes, *stage = row_stage + group * S::kBoxBytes;
+        uint32_t done = 0, bias_tq = 0xffffffffu;
         bool bad = false;
-        for (uint32_t u = blockIdx.x; u < P.units; u += gridDim.x) {
+        for (uint32_t u = first_unit; u < P.units; u += unit_step) {
             const Unit t = unit_of(P, u);
-            const uint32_t row0 = t.tp * kTileP + quarter * 32, row = row0 + lane;
-            const uint32_t col0 = t.tq * TN + half * kHalf;
-            const float *ps = P.p_scales + size_t(min(row, P.p_rows - 1) >> P.p_shift) * P.k_blocks;
-            // QROWS: this thread's column of the tile; else the warp's columns' scale
-            const uint32_t q_row = min(QROWS ? t.tq * TN + et : col0, P.q_rows - 1);
-            const float *qs = P.q_scales + size_t(q_row >> P.q_shift) * P.k_blocks;
-            float p_next = __ldg(ps + t.k0);
-            float q_next = (!QROWS || et < TN) ? __ldg(qs + t.k0) : 0.0f;
-            uint64_t acc[kHalf / 2];
+            const uint32_t row0 = (t.tp * S::kCtas + rank) * kTileP + quarter * 32, row = row0 + lane;
+            const uint32_t col0 = t.tq * TN + group * kCols;
+            uint64_t acc[kCols / 2];
+            if (!SWAP && P.bias && P.splits == 1) {
+                // the sums start from the bias
+                if (t.tq != bias_tq) {
+                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                    if (et < TN) bias_s[et] = t.tq * TN + et < P.q_rows ? bias_at(P, t.tq * TN + et) : 0.0f;
+                    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+                    bias_tq = t.tq;
+                }
 #pragma unroll
-            for (int i = 0; i < kHalf / 2; ++i) acc[i] = 0;
+                for (int i = 0; i < kCols / 2; ++i)
+                    acc[i] = *reinterpret_cast<const uint64_t *>(bias_s + group * kCols + 2 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
+            }
             for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++done) {
                 const uint32_t b = done % S::kAccs, turn = done / S::kAccs;
-                const float p_cur = p_next, q_cur = q_next;
-                float *q_buf = q_scale + (done & 1) * TN;
-                if (QROWS && et < TN) q_buf[et] = q_cur;
-                if (kb + 1 < t.k1) {
-                    p_next = __ldg(ps + kb + 1);
-                    if (!QROWS || et < TN) q_next = __ldg(qs + kb + 1);
-                }
+                const uint32_t ss = done % S::kScaleStages;
+                if (!mbar_wait(scale_full + 8 * ss, (done / S::kScaleStages) & 1, &abort_flag)) bad = true;
+                const float *sc = scales + ss * S::kScaleFloats;
+                const float *q_sc = sc + kTileP + (QROWS ? group * kCols : group);
+                const float one = QROWS ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * *q_sc;
                 if (!mbar_wait(acc_full + 8 * b, turn & 1, &abort_flag)) bad = true;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                if (QROWS) asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-                const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + half * kHalf;
-                const float one = QROWS ? p_cur : p_cur * q_cur;
+                const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
                 const uint64_t s2 = pair(one, one);
-                uint32_t r[2][kChunk];
-                tmem_load(r[0], addr);
 #pragma unroll
-                for (int c = 0; c < kHalf / kChunk; ++c) {
-                    tmem_wait(r[c & 1]);
-                    if (c + 1 < kHalf / kChunk) tmem_load(r[(c + 1) & 1], addr + (c + 1) * kChunk);
+                for (int c = 0; c < kCols / kChunk; ++c) {
+                    uint32_t v[kChunk];
+                    tmem_load(v, addr + c * kChunk);
+                    tmem_wait(v);
 #pragma unroll
-                    for (int i = 0; i < kChunk; i += 2) {
-                        const uint64_t x = pair(__uint_as_float(r[c & 1][i]), __uint_as_float(r[c & 1][i + 1]));
-                        uint64_t s = s2;
-                        if (QROWS)
-                            s = mul_pair(s2, *reinterpret_cast<const uint64_t *>(q_buf + half * kHalf + c * kChunk + i));
-                        fma_pair(acc[(c * kChunk + i) / 2], x, s);
+                    for (int i = 0; i < kChunk; i += 4) {
+                        const uint64_t x = pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        const uint64_t y = pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                        uint64_t sx = s2, sy = s2;
+                        if (QROWS) {
+                            const float4 q = *reinterpret_cast<const float4 *>(q_sc + c * kChunk + i);
+                            sx = mul_pair(s2, pair(q.x, q.y));
+                            sy = mul_pair(s2, pair(q.z, q.w));
+                        }
+                        fma_pair(acc[(c * kChunk + i) / 2], x, sx);
+                        fma_pair(acc[(c * kChunk + i) / 2 + 1], y, sy);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8 * b);
+                if (lane == 0) {
+                    arrive_at_first<PAIR>(acc_empty + 8 * b);
+                    mbar_arrive(scale_empty + 8 * ss);
+                }
             }
             if (bad) {
 #pragma unroll
-                for (int i = 0; i < kHalf / 2; ++i) acc[i] = 0x7fc000007fc00000ull;
+                for (int i = 0; i < kCols / 2; ++i) acc[i] = 0x7fc000007fc00000ull;
             }
             if (P.splits > 1) {
-                float4 *dst = P.parts + ((size_t(u) * kEpiWarps + (warp - 2)) * (kHalf / 4)) * 32 + lane;
+                const size_t block = PAIR ? size_t(u) * 2 + rank : u;
+                float4 *dst = P.parts + ((block * kEpiWarps + (warp - 4)) * (kCols / 4)) * 32 + lane;
 #pragma unroll
-                for (int i = 0; i < kHalf / 4; ++i) {
+                for (int i = 0; i < kCols / 4; ++i) {
                     const float2 x = unpair(acc[2 * i]), y = unpair(acc[2 * i + 1]);
                     dst[i * 32] = make_float4(x.x, x.y, y.x, y.y);
                 }
-                continue;
-            }
-            if (SWAP) {
+            } else if constexpr (SWAP) {
                 // lane = column of out: the warp writes 32 consecutive elements
                 const float bias = P.bias && row < P.p_rows ? bias_at(P, row) : 0.0f;
 #pragma unroll
-                for (int i = 0; i < kHalf / 2; ++i) {
+                for (int i = 0; i < kCols / 2; ++i) {
                     const float2 x = unpair(acc[i]);
                     if (row < P.p_rows && col0 + 2 * i < P.q_rows)
                         store_value(P.out, P.out_dtype, uint64_t(col0 + 2 * i) * P.ldo + row, x.x + bias);
                     if (row < P.p_rows && col0 + 2 * i + 1 < P.q_rows)
                         store_value(P.out, P.out_dtype, uint64_t(col0 + 2 * i + 1) * P.ldo + row, x.y + bias);
                 }
-                continue;
-            }
-            if (P.bias) {
-#pragma unroll
-                for (int i = 0; i < kHalf / 2; ++i) {
-                    const uint32_t n = col0 + 2 * i;
-                    const float2 x = unpair(acc[i]);
-                    acc[i] = pair(x.x + (n < P.q_rows ? bias_at(P, n) : 0.0f),
-                                  x.y + (n + 1 < P.q_rows ? bias_at(P, n + 1) : 0.0f));
-                }
-            }
-            if constexpr (kHalf >= 32) {
-                if (P.out_dtype == SDFOAM_F32) {
-#pragma unroll
-                    for (int c = 0; c < kHalf / 16; ++c) {
-                        if (col0 + c * 16 >= P.q_rows || row0 >= P.p_rows) continue;  // the same for every lane
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float2 x = unpair(acc[c * 8 + i]);
-                            w[2 * i] = __float_as_uint(x.x);
-                            w[2 * i + 1] = __float_as_uint(x.y);
-                        }
-                        store_box(P, &map_out, box, w, row0, col0 + c * 16, lane);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < kHalf / 32; ++c) {
-                        if (col0 + c * 32 >= P.q_rows || row0 >= P.p_rows) continue;
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 x = unpair(acc[c * 16 + i]);
-                            w[i] = pack2(P.out_dtype, x.x, x.y);
-                        }
-                        store_box(P, &map_out, box, w, row0, col0 + c * 32, lane);
-                    }
-                }
+            } else if constexpr (kCols >= 32) {
+                store_rows<kCols, S::kGroups>(P, &map_out, stage, row_stage, acc, row0, col0, lane, group, quarter);
             } else if (row < P.p_rows) {
                 // at most 16 columns per thread
 #pragma unroll
-                for (int i = 0; i < kHalf / 2; ++i) {
+                for (int i = 0; i < kCols / 2; ++i) {
                     const float2 x = unpair(acc[i]);
                     const uint64_t at = uint64_t(row) * P.ldo + col0 + 2 * i;
                     if (col0 + 2 * i < P.q_rows) store_value(P.out, P.out_dtype, at, x.x);
@@ -448,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                 }
             }
         }
-        // the TMA stores have read their boxes and are complete
+        // the bulk stores are complete
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncthreads();
@@ -456,24 +673,30 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
         *static_cast<volatile int *>(P.error) = 1;
         __threadfence_system();
     }
+    // the other CTA's copies, commits and arrivals are done before either leaves
+    if constexpr (PAIR) cluster_sync();
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols));
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols));
     }
 }
 
-// Adds the slices of a tile in order (parts: [tile][slice][warp][columns / 4]
-// [lane] float4, the epilogue's own order) and the bias; also the product
-// with an empty reduction (no slices).
-template <int TN, bool SWAP>
+// Adds the slices of a tile in order (parts: [tile][slice][CTA][warp]
+// [columns / 4][lane] float4, the epilogue's own order) and the bias.
+template <int TN, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(256) join_slices_kernel(const BlockParams P) {
-    constexpr int kHalf = TN / 2;
-    constexpr uint32_t kPerTile = kEpiWarps * (kHalf / 4) * 32;
+    using S = Shape<TN, PAIR>;
+    constexpr int kCols = S::kCols, kCtas = S::kCtas;
+    constexpr uint32_t kPerCta = kEpiWarps * (kCols / 4) * 32, kPerTile = kPerCta * kCtas;
     const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
     const uint32_t tile = uint32_t(i / kPerTile), in = uint32_t(i % kPerTile);
     if (tile >= P.tiles_p * P.tiles_q) return;
-    const uint32_t lane = in & 31, c4 = (in >> 5) % (kHalf / 4), w = (in >> 5) / (kHalf / 4);
+    const uint32_t rank = in / kPerCta;
+    const uint32_t lane = in & 31, c4 = (in >> 5) % (kCols / 4), w = (in % kPerCta >> 5) / (kCols / 4);
     const Unit t = unit_of(P, tile * P.splits);
     const float4 *src = P.parts + size_t(tile) * P.splits * kPerTile + in;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -485,9 +708,8 @@ __global__ void __launch_bounds__(256) join_slices_kernel(const BlockParams P) {
         v[2] += x.z;
         v[3] += x.w;
     }
-    // warp w of the epilogue: TMEM quarter (w + 2) % 4, half w / 4
-    const uint32_t row = t.tp * kTileP + ((w + 2) & 3) * 32 + lane;
-    const uint32_t col = t.tq * TN + (w / 4) * kHalf + c4 * 4;
+    const uint32_t row = (t.tp * kCtas + rank) * kTileP + (w & 3) * 32 + lane;  // warp w of the epilogue: quarter w % 4, group w / 4
+    const uint32_t col = t.tq * TN + (w / 4) * kCols + c4 * 4;
     if (row >= P.p_rows) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -511,7 +733,7 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(const BlockParams P, uin
 // --------------------------------------------------------------------------
 
 struct Plan {
-    bool swap;
+    bool swap, pair;
     int tn;
     uint32_t tiles_p, tiles_q, k_blocks, splits;
 };
@@ -525,8 +747,11 @@ Plan plan_of(uint32_t m, uint32_t n, uint32_t k) {
     if (l.tn == 256 && uint64_t(l.tiles_p) * ((q + 255) / 256) < kSms) l.tn = 128;
     l.tiles_q = (q + l.tn - 1) / l.tn;
     l.k_blocks = (k + kBlockK - 1) / kBlockK;
-    const uint64_t tiles = uint64_t(l.tiles_p) * l.tiles_q;
-    l.splits = tiles < kSms ? std::min<uint32_t>(l.k_blocks, uint32_t(kSms / tiles)) : 1;
+    uint64_t tiles = uint64_t(l.tiles_p) * l.tiles_q;
+    // pairs where there is a tile of 256 x 256 for each of them
+    l.pair = l.tn == 256;
+    if (l.pair) l.tiles_p = (l.tiles_p + 1) / 2;
+    l.splits = !l.pair && tiles < kSms ? std::min<uint32_t>(l.k_blocks, uint32_t(kSms / tiles)) : 1;
     return l;
 }
 
@@ -543,44 +768,62 @@ bool operand_map(CUtensorMap *map, const void *base, uint32_t rows, uint32_t k, 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// out [rows, cols] in boxes of 32 rows x 64 bytes, 64-byte swizzle.
-bool output_map(CUtensorMap *map, void *base, uint32_t rows, uint32_t cols, uint64_t ld, uint32_t dtype) {
+// out [rows, cols] in boxes of 32 rows x 128 bytes (64 for tiles of 32 16-bit
+// columns per warp), swizzled over the same width.
+bool output_map(CUtensorMap *map, void *base, uint32_t rows, uint32_t cols, uint64_t ld, uint32_t dtype, int tn) {
     auto fn = encode_fn();
     if (!fn) return false;
     const uint32_t size = dtype == SDFOAM_F32 ? 4 : 2;
     const cuuint64_t dims[2] = {cols, rows};
     const cuuint64_t strides[1] = {ld * size};
-    const cuuint32_t box[2] = {64 / size, 32};
+    const uint32_t bytes = dtype != SDFOAM_F32 && tn == 64 ? 64 : 128;
+    const cuuint32_t box[2] = {bytes / size, 32};
     const cuuint32_t elem[2] = {1, 1};
     return fn(map, dtype == SDFOAM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base,
-              dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+              dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int TN, bool QROWS, bool SWAP>
+template <int TN, bool QROWS, bool SWAP, bool PAIR>
 cudaError_t launch_tiles(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mo, const BlockParams &P,
                          cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(block_mm_kernel<TN, QROWS, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         int(Shape<TN>::kSmem));
+    using S = Shape<TN, PAIR>;
+    auto kernel = block_mm_kernel<TN, QROWS, SWAP, PAIR>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem));
     if (e != cudaSuccess) return e;
-    block_mm_kernel<TN, QROWS, SWAP><<<std::min<uint32_t>(P.units, kSms), kThreads, Shape<TN>::kSmem, stream>>>(mp, mq, mo, P);
-    if ((e = cudaGetLastError()) != cudaSuccess || P.splits == 1) return e;
-    const uint64_t threads = uint64_t(P.tiles_p) * P.tiles_q * kTileP * TN / 4;
-    join_slices_kernel<TN, SWAP><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(P);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min<uint32_t>(P.units, kSms / S::kCtas) * S::kCtas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S::kCtas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    if ((e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, mo, P)) != cudaSuccess || P.splits == 1) return e;
+    const uint64_t threads = uint64_t(P.tiles_p) * P.tiles_q * S::kCtas * kTileP * TN / 4;
+    join_slices_kernel<TN, SWAP, PAIR><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(P);
     return cudaGetLastError();
 }
 
 template <int TN>
-cudaError_t launch_tn(bool swap, const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mo,
+cudaError_t launch_tn(const Plan &l, const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mo,
                       const BlockParams &P, cudaStream_t stream) {
+    const bool rows = P.q_shift == 0;
     if constexpr (TN <= 64) {
-        if (swap) {
-            if (P.q_shift == 0) return launch_tiles<TN, true, true>(mp, mq, mo, P, stream);
-            return launch_tiles<TN, false, true>(mp, mq, mo, P, stream);
-        }
+        if (l.swap)
+            return rows ? launch_tiles<TN, true, true, false>(mp, mq, mo, P, stream)
+                        : launch_tiles<TN, false, true, false>(mp, mq, mo, P, stream);
     }
-    if (P.q_shift == 0) return launch_tiles<TN, true, false>(mp, mq, mo, P, stream);
-    return launch_tiles<TN, false, false>(mp, mq, mo, P, stream);
+    if constexpr (TN == 256)
+        return rows ? launch_tiles<TN, true, false, true>(mp, mq, mo, P, stream)
+                    : launch_tiles<TN, false, false, true>(mp, mq, mo, P, stream);
+    else
+        return rows ? launch_tiles<TN, true, false, false>(mp, mq, mo, P, stream)
+                    : launch_tiles<TN, false, false, false>(mp, mq, mo, P, stream);
 }
 
 }  // namespace
@@ -588,12 +831,13 @@ cudaError_t launch_tn(bool swap, const CUtensorMap &mp, const CUtensorMap &mq, c
 size_t block_matmul_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
     if (m == 0 || n == 0 || k == 0) return 0;
     const Plan l = plan_of(m, n, k);
-    return l.splits > 1 ? size_t(l.tiles_p) * l.tiles_q * l.splits * kTileP * l.tn * 4 : 0;
+    return l.splits > 1 ? size_t(l.tiles_p) * l.tiles_q * l.splits * (l.pair ? 2 : 1) * kTileP * l.tn * 4 : 0;
 }
 
-cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint32_t m,
-                                const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint32_t n,
-                                uint32_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
+cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
+                                uint64_t a_scale_block, int a_block_rows, uint32_t m, const void *b, uint64_t ldb,
+                                const float *b_scales, uint64_t b_scale_row, uint64_t b_scale_block, int b_block_rows,
+                                uint32_t n, uint32_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
                                 uint32_t out_dtype, void *workspace, int *error, cudaStream_t stream) {
     if (m == 0 || n == 0) return cudaSuccess;
     BlockParams P{};
@@ -616,23 +860,31 @@ cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scal
     P.units = l.tiles_p * l.tiles_q * l.splits;
     P.p_scales = l.swap ? b_scales : a_scales;
     P.q_scales = l.swap ? a_scales : b_scales;
+    P.p_scale_row = l.swap ? b_scale_row : a_scale_row;
+    P.p_scale_block = l.swap ? b_scale_block : a_scale_block;
+    P.q_scale_row = l.swap ? a_scale_row : b_scale_row;
+    P.q_scale_block = l.swap ? a_scale_block : b_scale_block;
     P.p_shift = (l.swap ? b_block_rows : a_block_rows) == 128 ? 7 : 0;
     P.q_shift = (l.swap ? a_block_rows : b_block_rows) == 128 ? 7 : 0;
     P.parts = static_cast<float4 *>(workspace);
     P.error = error;
     const uint32_t size = out_dtype == SDFOAM_F32 ? 4 : 2;
-    P.box_store = !l.swap && l.splits == 1 && l.tn >= 64 && ((reinterpret_cast<uintptr_t>(out) | (ldo * size)) & 15u) == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(out);
+    P.store = l.tn < 64 || l.swap || l.splits > 1                   ? kStoreRows
+              : ((at | (ldo * size)) & 15u) == 0                   ? kStoreBox
+              : size == 2 && l.tiles_q == 1 && ldo == n && !(at & 15u) ? kStoreSpan
+                                                                   : kStoreRows;
     CUtensorMap mp, mq, mo{};
     if (!operand_map(&mp, l.swap ? b : a, P.p_rows, k, l.swap ? ldb : lda, kTileP) ||
-        !operand_map(&mq, l.swap ? a : b, P.q_rows, k, l.swap ? lda : ldb, uint32_t(l.tn)) ||
-        (P.box_store && !output_map(&mo, out, m, n, ldo, out_dtype)))
+        !operand_map(&mq, l.swap ? a : b, P.q_rows, k, l.swap ? lda : ldb, uint32_t(l.pair ? l.tn / 2 : l.tn)) ||
+        (P.store == kStoreBox && !output_map(&mo, out, m, n, ldo, out_dtype, l.tn)))
         return cudaErrorInvalidValue;
     switch (l.tn) {
-        case 16: return launch_tn<16>(l.swap, mp, mq, mo, P, stream);
-        case 32: return launch_tn<32>(l.swap, mp, mq, mo, P, stream);
-        case 64: return launch_tn<64>(l.swap, mp, mq, mo, P, stream);
-        case 128: return launch_tn<128>(l.swap, mp, mq, mo, P, stream);
-        default: return launch_tn<256>(l.swap, mp, mq, mo, P, stream);
+        case 16: return launch_tn<16>(l, mp, mq, mo, P, stream);
+        case 32: return launch_tn<32>(l, mp, mq, mo, P, stream);
+        case 64: return launch_tn<64>(l, mp, mq, mo, P, stream);
+        case 128: return launch_tn<128>(l, mp, mq, mo, P, stream);
+        default: return launch_tn<256>(l, mp, mq, mo, P, stream);
     }
 }
 

@@ -13,7 +13,9 @@
 // A training step needs a matrix twice: in rows for the product and turned
 // for the weight gradient, whose reduction runs over the rows, with blocks
 // along that axis.  One pass over 128 x 128 tiles in registers writes either
-// or both, so the input is read once.  HBM bounds it (2 or 4 bytes in, one
+// or both, so the input is read once.  Scales are stored block by block, the
+// rows of one block of columns next to each other, as a product's tile reads
+// them.  HBM bounds it (2 or 4 bytes in, one
 // or two out per element).
 #include <algorithm>
 
@@ -129,8 +131,8 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
         for (int w = 0; w < 8; ++w) top = max(top, top_all[w]);
         whole = scale_exponent(top);
         if (threadIdx.x == 0) {
-            if (NORMAL) P.scales[size_t(mb) * P.k_blocks + kb] = scale_value(whole);
-            if (TURNED) P.turned_scales[size_t(kb) * P.m_blocks + mb] = scale_value(whole);
+            if (NORMAL) P.scales[size_t(kb) * P.m_blocks + mb] = scale_value(whole);
+            if (TURNED) P.turned_scales[size_t(mb) * P.k_blocks + kb] = scale_value(whole);
         }
     }
 
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
             }
             const float inv = scale_inverse(exponent);
             if (row0 + r < P.m) {
-                if (BLOCK_ROWS == 1 && c == 0) P.scales[size_t(row0 + r) * P.k_blocks + kb] = scale_value(exponent);
+                if (BLOCK_ROWS == 1 && c == 0) P.scales[size_t(kb) * P.m + row0 + r] = scale_value(exponent);
                 // whole 16-byte pieces of the row are written, zeros past k
                 if (col0 < ((P.k + 15u) & ~15u)) {
                     uint2 q;
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
             if (g == 0) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (i < left) P.turned_scales[size_t(col0 + i) * P.m_blocks + mb] = scale_value(exponent[i]);
+                    if (i < left) P.turned_scales[size_t(mb) * P.k + col0 + i] = scale_value(exponent[i]);
             }
         } else {
 #pragma unroll
@@ -249,7 +251,8 @@ constexpr int kDequantItems = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const unsigned char *__restrict__ values, size_t ldv,
                                                               const float *__restrict__ scales, uint32_t shift,
-                                                              uint32_t k_blocks, uint32_t m, uint32_t k, uint32_t units,
+                                                              size_t scale_row, size_t scale_block, uint32_t m,
+                                                              uint32_t k, uint32_t units,
                                                               T *__restrict__ out) {
     const uint64_t total = uint64_t(m) * units;
     const uint64_t first = uint64_t(blockIdx.x) * (kThreads * kDequantItems);
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const unsigned cha
         if (first + e >= total) return;
         const uint32_t r = (col0 + e) / units, u = (col0 + e) - r * units, col = u * VEC;
         const uint64_t row = row0 + r;
-        const float s = __ldg(scales + (row >> shift) * k_blocks + (col >> 7));
+        const float s = __ldg(scales + (row >> shift) * scale_row + (col >> 7) * scale_block);
         const unsigned char *src = values + row * ldv + col;
         T *dst = out + row * k + col;
         if (VEC == 4) {
@@ -293,16 +296,16 @@ void quantize_typed(const QuantParams &P, int block_rows, unsigned blocks, cudaS
 }
 
 template <typename T>
-void dequantize_typed(const void *values, size_t ldv, const float *scales, int block_rows, uint32_t m, uint32_t k,
-                      void *out, cudaStream_t stream) {
+void dequantize_typed(const void *values, size_t ldv, const float *scales, size_t scale_row, size_t scale_block,
+                      int block_rows, uint32_t m, uint32_t k, void *out, cudaStream_t stream) {
     const bool vec = k % 4 == 0 && ldv % 4 == 0 && (reinterpret_cast<uintptr_t>(values) & 3u) == 0 &&
                      (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
-    const uint32_t units = vec ? k / 4 : k, shift = block_rows == 128 ? 7 : 0, kb = (k + 127) / 128;
+    const uint32_t units = vec ? k / 4 : k, shift = block_rows == 128 ? 7 : 0;
     const uint64_t per = kThreads * kDequantItems;
     const unsigned blocks = unsigned((uint64_t(m) * units + per - 1) / per);
     const unsigned char *v = static_cast<const unsigned char *>(values);
-    if (vec) dequantize_kernel<T, 4><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, kb, m, k, units, static_cast<T *>(out));
-    else dequantize_kernel<T, 1><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, kb, m, k, units, static_cast<T *>(out));
+    if (vec) dequantize_kernel<T, 4><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
+    else dequantize_kernel<T, 1><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
 }
 
 }  // namespace
@@ -333,13 +336,14 @@ cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint
     return cudaGetLastError();
 }
 
-cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, int block_rows, uint32_t m,
-                                    uint32_t k, uint32_t dtype, void *out, cudaStream_t stream) {
+cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, size_t scale_row,
+                                    size_t scale_block, int block_rows, uint32_t m, uint32_t k, uint32_t dtype,
+                                    void *out, cudaStream_t stream) {
     if (m == 0 || k == 0) return cudaSuccess;
     switch (dtype) {
-        case SDFOAM_F32: dequantize_typed<float>(values, ldv, scales, block_rows, m, k, out, stream); break;
-        case SDFOAM_F16: dequantize_typed<__half>(values, ldv, scales, block_rows, m, k, out, stream); break;
-        default: dequantize_typed<__nv_bfloat16>(values, ldv, scales, block_rows, m, k, out, stream); break;
+        case SDFOAM_F32: dequantize_typed<float>(values, ldv, scales, scale_row, scale_block, block_rows, m, k, out, stream); break;
+        case SDFOAM_F16: dequantize_typed<__half>(values, ldv, scales, scale_row, scale_block, block_rows, m, k, out, stream); break;
+        default: dequantize_typed<__nv_bfloat16>(values, ldv, scales, scale_row, scale_block, block_rows, m, k, out, stream); break;
     }
     return cudaGetLastError();
 }

@@ -682,8 +682,9 @@ int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_quantize");
 }
 
-int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, int block_rows, uint64_t m,
-                            uint64_t k, uint32_t dtype, void *out, sdfoam_stream_t stream) {
+int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, uint64_t scale_row,
+                            uint64_t scale_block, int block_rows, uint64_t m, uint64_t k, uint32_t dtype, void *out,
+                            sdfoam_stream_t stream) {
     int rc = check_blocks(m, k, block_rows);
     if (rc != SDFOAM_OK) return rc;
     if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
@@ -691,8 +692,9 @@ int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scale
         return fail(SDFOAM_ERR_INVALID, "values, scales and out must be non-NULL");
     if (ldv < k || (ldv >> 40)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
     if (!aligned_to(out, dtype)) return fail(SDFOAM_ERR_INVALID, "out must be aligned to its elements");
-    cudaError_t e = launch_block_dequantize(values, ldv, scales, block_rows, static_cast<uint32_t>(m),
-                                            static_cast<uint32_t>(k), dtype, out, reinterpret_cast<cudaStream_t>(stream));
+    cudaError_t e = launch_block_dequantize(values, ldv, scales, scale_row, scale_block, block_rows,
+                                            static_cast<uint32_t>(m), static_cast<uint32_t>(k), dtype, out,
+                                            reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_dequantize");
 }
 
@@ -701,10 +703,12 @@ size_t sdfoam_block_matmul_workspace_bytes(uint64_t m, uint64_t n, uint64_t k) {
     return block_matmul_workspace_bytes(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(k));
 }
 
-int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint64_t m,
-                        const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint64_t n, uint64_t k,
-                        const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo, uint32_t out_dtype,
-                        void *workspace, size_t workspace_bytes, int *error, sdfoam_stream_t stream) {
+int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
+                        uint64_t a_scale_block, int a_block_rows, uint64_t m, const void *b, uint64_t ldb,
+                        const float *b_scales, uint64_t b_scale_row, uint64_t b_scale_block, int b_block_rows,
+                        uint64_t n, uint64_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
+                        uint32_t out_dtype, void *workspace, size_t workspace_bytes, int *error,
+                        sdfoam_stream_t stream) {
     int rc = check_blocks(m, k, a_block_rows);
     if (rc == SDFOAM_OK) rc = check_blocks(n, k, b_block_rows);
     if (rc == SDFOAM_OK) rc = check_blocks(m, n, 1);
@@ -722,7 +726,8 @@ int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, int 
     const size_t need = sdfoam_block_matmul_workspace_bytes(m, n, k);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(SDFOAM_ERR_INVALID, "workspace is too small or not 16-byte aligned");
-    cudaError_t e = launch_block_matmul(a, lda, a_scales, a_block_rows, static_cast<uint32_t>(m), b, ldb, b_scales,
+    cudaError_t e = launch_block_matmul(a, lda, a_scales, a_scale_row, a_scale_block, a_block_rows,
+                                        static_cast<uint32_t>(m), b, ldb, b_scales, b_scale_row, b_scale_block,
                                         b_block_rows, static_cast<uint32_t>(n), static_cast<uint32_t>(k), bias,
                                         bias_dtype, out, ldo, out_dtype, workspace, error,
                                         reinterpret_cast<cudaStream_t>(stream));

@@ -102,12 +102,14 @@ cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t co
 cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint32_t m, uint32_t k, int block_rows,
                                   void *values, size_t ldv, float *scales, void *turned, size_t ldt,
                                   float *turned_scales, cudaStream_t stream);
-cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, int block_rows, uint32_t m,
-                                    uint32_t k, uint32_t dtype, void *out, cudaStream_t stream);
+cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, size_t scale_row,
+                                    size_t scale_block, int block_rows, uint32_t m, uint32_t k, uint32_t dtype,
+                                    void *out, cudaStream_t stream);
 size_t block_matmul_workspace_bytes(uint32_t m, uint32_t n, uint32_t k);
-cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, int a_block_rows, uint32_t m,
-                                const void *b, uint64_t ldb, const float *b_scales, int b_block_rows, uint32_t n,
-                                uint32_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
+cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
+                                uint64_t a_scale_block, int a_block_rows, uint32_t m, const void *b, uint64_t ldb,
+                                const float *b_scales, uint64_t b_scale_row, uint64_t b_scale_block, int b_block_rows,
+                                uint32_t n, uint32_t k, const void *bias, uint32_t bias_dtype, void *out, uint64_t ldo,
                                 uint32_t out_dtype, void *workspace, int *error, cudaStream_t stream);
 
 // Gradient workspace layout:

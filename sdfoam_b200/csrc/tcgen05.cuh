@@ -61,10 +61,11 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 
 // Polls the phase of the given parity.  False when *abort is raised or after
 // kWaitNs nanoseconds (which raises *abort); abort == nullptr: only the time
-// bound (the clean-up waits).  A phase that is already complete costs one
-// poll and no clock reading.
+// bound (the clean-up waits).  The clock is read only after some polls: a
+// tile's wait is over by then.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
-    if (mbar_try(bar, parity)) return true;
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     for (uint32_t i = 0; i < kMaxPolls; ++i) {
         if (mbar_try(bar, parity)) return true;

@@ -134,7 +134,8 @@ def test_quantize_edges(block_rows):
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 4096, 4096), (2, 217, 39), (7, 300, 1000), (16, 256, 256), (17, 129, 130),
          (33, 1000, 257), (64, 65, 127), (64, 64, 64), (65, 64, 128), (100, 100, 100), (128, 256, 384), (129, 257, 513),
          (300, 1, 500), (1000, 16, 256), (1000, 31, 47), (1500, 64, 2000), (2000, 217, 256), (777, 1111, 333),
-         (256, 256, 20001), (5000, 3000, 128), (20000, 512, 300)]
+         (256, 256, 20001), (5000, 3000, 128), (20000, 512, 300), (20001, 217, 300), (19100, 250, 129),
+         (40000, 100, 256), (40001, 63, 257)]
 
 
 @pytest.mark.gpu
@@ -406,14 +407,14 @@ def test_entry_points_refuse_bad_arguments():
     assert quantize(m=0, x=None, v=None) == 0
 
     def dequantize(v=p, ldv=32, s=p, rows=1, m=4, k=32, dtype=0, out=p):
-        return lib.sdfoam_block_dequantize(v, ldv, s, rows, m, k, dtype, out, None)
+        return lib.sdfoam_block_dequantize(v, ldv, s, 1, 1, rows, m, k, dtype, out, None)
 
     assert dequantize(rows=0) == 1 and dequantize(dtype=5) == 2 and dequantize(ldv=31) == 1
     assert dequantize(out=None) == 1 and dequantize(out=ctypes.c_void_p(4098)) == 1
 
     def matmul(a=p, lda=128, sa=p, ra=1, m=300, b=p, ldb=128, sb=p, rb=128, n=256, k=128, bias=None, bt=0, out=p,
                ldo=256, ot=2, ws=p, size=1 << 30, error=p):
-        return lib.sdfoam_block_matmul(a, lda, sa, ra, m, b, ldb, sb, rb, n, k, bias, bt, out, ldo, ot, ws, size, error,
+        return lib.sdfoam_block_matmul(a, lda, sa, 1, 1, ra, m, b, ldb, sb, 1, 1, rb, n, k, bias, bt, out, ldo, ot, ws, size, error,
                                        None)
 
     assert matmul(ra=3) == 1 and matmul(rb=64) == 1 and matmul(ot=3) == 2 and matmul(bias=p, bt=4) == 2
