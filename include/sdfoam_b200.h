@@ -486,7 +486,10 @@ SDFOAM_API int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, u
  *     [ceil(k / 128), ceil(m / block_rows)], the rows' scales of one block of
  *     columns after another (NULL: not written); turned [k, ldt] and
  *     turned_scales [ceil(m / 128), ceil(k / block_rows)] are the same of x^T,
- *     its blocks along x's rows (NULL: not written).  ldv and ldt
+ *     its blocks along x's rows (NULL: not written).  With turned,
+ *     column_sums [k] of sums_dtype (NULL: not written) are the sums of x's
+ *     columns, fp32 in a fixed order (a bias's gradient), over a workspace of
+ *     ceil(m / 128) * k floats.  ldv and ldt
  *     are multiples of 16 of at least k and m, values and turned 16-byte
  *     aligned; columns up to the next multiple of 16 are written as zeros.
  *   dequantize: out [m, k] contiguous of dtype = values * scales, the scale of
@@ -494,7 +497,8 @@ SDFOAM_API int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, u
  * m and k below 2^31; ceil(m / 128) * ceil(k / 128) below 2^31. */
 SDFOAM_API int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m, uint64_t k,
                                      int block_rows, void *values, uint64_t ldv, float *scales, void *turned,
-                                     uint64_t ldt, float *turned_scales, sdfoam_stream_t stream);
+                                     uint64_t ldt, float *turned_scales, void *column_sums, uint32_t sums_dtype,
+                                     float *workspace, sdfoam_stream_t stream);
 SDFOAM_API int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scales, uint64_t scale_row,
                                        uint64_t scale_block, int block_rows, uint64_t m, uint64_t k, uint32_t dtype,
                                        void *out, sdfoam_stream_t stream);

@@ -257,7 +257,7 @@ def load():
     lib.sdfoam_lookup_rows_backward.restype = ctypes.c_int
     lib.sdfoam_lookup_rows_backward.argtypes = [vp, u32, u64, u32, vp, u64, u32, f32, vp, u32, vp, ctypes.c_size_t, vp]
     lib.sdfoam_block_quantize.restype = ctypes.c_int
-    lib.sdfoam_block_quantize.argtypes = [vp, u64, u32, u64, u64, i32, vp, u64, vp, vp, u64, vp, vp]
+    lib.sdfoam_block_quantize.argtypes = [vp, u64, u32, u64, u64, i32, vp, u64, vp, vp, u64, vp, vp, u32, vp, vp]
     lib.sdfoam_block_dequantize.restype = ctypes.c_int
     lib.sdfoam_block_dequantize.argtypes = [vp, u64, vp, u64, u64, i32, u64, u64, u32, vp, vp]
     lib.sdfoam_block_matmul_workspace_bytes.restype = ctypes.c_size_t

@@ -74,8 +74,9 @@ def _values(rows: int, columns: int, device) -> torch.Tensor:
     return v if ld == columns else v[:, :columns]
 
 
-def _quantize(x, block_rows, normal, turned):
-    """(values, scales) or None of x and of x turned."""
+def _quantize(x, block_rows, normal, turned, sums=None):
+    """(values, scales) or None of x and of x turned; the sums of x's columns
+    go to the vector ``sums`` (only with turned)."""
     x = _matrix(x)
     m, k = x.shape
     dev = x.device
@@ -86,13 +87,20 @@ def _quantize(x, block_rows, normal, turned):
     if turned:
         vt = _values(k, m, dev)
         st = torch.empty((_blocks(m), k if block_rows == 1 else _blocks(k)), dtype=torch.float32, device=dev).t()
+    ws = None
+    if sums is not None:
+        if m == 0:
+            sums.zero_()
+        ws = torch.empty((_blocks(m), k), dtype=torch.float32, device=dev)
     lib = _lib.load()
     with torch.cuda.device(dev):
         _lib.check(lib.sdfoam_block_quantize(
             x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, k, block_rows,
             v.data_ptr() if normal else None, max(v.stride(0), k) if normal else 0, s.data_ptr() if normal else None,
             vt.data_ptr() if turned else None, max(vt.stride(0), m) if turned else 0,
-            st.data_ptr() if turned else None, torch.cuda.current_stream().cuda_stream))
+            st.data_ptr() if turned else None, None if sums is None else sums.data_ptr(),
+            0 if sums is None else _DTYPES[sums.dtype], None if ws is None else ws.data_ptr(),
+            torch.cuda.current_stream().cuda_stream))
     return (v, s) if normal else None, (vt, st) if turned else None
 
 
@@ -227,14 +235,14 @@ class _BlockLinear(torch.autograd.Function):
         qt, qts, wt, wts = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
         dx = dw = db = None
-        if need_x or need_w:
-            g, gt = _quantize(grad, 1, need_x, need_w)
-            if need_x:
-                dx = _product(*g, 1, wt, wts, _BLOCK, None, ctx.dtypes[0])
-            if need_w:
-                dw = _product(*gt, 1, qt, qts, 1, None, ctx.dtypes[1])
         if need_b:
-            db = grad.sum(0, dtype=torch.float32).to(ctx.dtypes[2])
+            db = torch.empty((grad.shape[1],), dtype=ctx.dtypes[2], device=grad.device)
+        # one pass over dy: its values for both products and its column sums
+        g, gt = _quantize(grad, 1, need_x, need_w or need_b, db)
+        if need_x:
+            dx = _product(*g, 1, wt, wts, _BLOCK, None, ctx.dtypes[0])
+        if need_w:
+            dw = _product(*gt, 1, qt, qts, 1, None, ctx.dtypes[1])
         return dx, dw, db
 
 

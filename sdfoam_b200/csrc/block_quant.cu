@@ -29,9 +29,9 @@ namespace sdfoam_b200 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr uint32_t kTile = 128;
-constexpr int kRows = 8;  // rows and columns of a thread's piece of the tile
+constexpr int kRows = 4;  // of a thread's piece of the tile, 8 columns wide
 
 struct QuantParams {
     const void *x;
@@ -40,28 +40,21 @@ struct QuantParams {
     unsigned char *values, *turned;  // [m, ldv], [k, ldt]; either may be null
     size_t ldv, ldt;
     float *scales, *turned_scales;
+    float *sums;                     // [ceil(m / 128), k] or null: sums of 128 rows
     uint32_t k_blocks, m_blocks;     // ceil(k / 128), ceil(m / 128)
 };
 
-// Scale of a block from the bits of its largest magnitude, as the bits of
-// the scale's exponent: 448 = 1.75 * 2^8, so the scale is 2^(e - 8) when the
-// magnitude 2^e * f has f <= 1.75 and 2^(e - 7) above.
-__device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) {
-    if (largest == 0) return 127;
-    const int e = int(largest >> 23) - 8 + ((largest & 0x7fffffu) > 0x600000u ? 1 : 0);
+// Scale of a block from its largest magnitude, as the bits of the scale's
+// exponent: 448 = 1.75 * 2^8, so the scale is 2^(e - 8) when the magnitude
+// 2^e * f has f <= 1.75 and 2^(e - 7) above.
+__device__ __forceinline__ uint32_t scale_exponent(float largest) {
+    const uint32_t bits = __float_as_uint(largest);
+    if (bits == 0) return 127;
+    const int e = int(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < 1 ? 1u : uint32_t(e);
 }
 __device__ __forceinline__ float scale_value(uint32_t exponent) { return __uint_as_float(exponent << 23); }
 __device__ __forceinline__ float scale_inverse(uint32_t exponent) { return __uint_as_float((254u - exponent) << 23); }
-
-// The magnitude's bits, 0 for infinities and NaN.
-__device__ __forceinline__ uint32_t magnitude(float v) {
-    const uint32_t a = __float_as_uint(v) & 0x7fffffffu;
-    return a < 0x7f800000u ? a : 0u;
-}
-
-// v / scale; NaN for infinities and NaN (v - v is 0 for every other v).
-__device__ __forceinline__ float scaled(float v, float inverse) { return fmaf(v, inverse, v - v); }
 
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -77,11 +70,11 @@ __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162f
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T *src, int left, float *v) {
     if (VEC && left >= 8) {
-        union {
+        union Eight {
             uint4 q[sizeof(T) / 2];
             T e[8];
-            __device__ uint4 &operator[](int i) { return q[i]; }
-        } u = {};
+            __device__ Eight() {}
+        } u;
 #pragma unroll
         for (int i = 0; i < int(sizeof(T) / 2); ++i) u.q[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
 #pragma unroll
@@ -92,16 +85,19 @@ __device__ __forceinline__ void load8(const T *src, int left, float *v) {
     }
 }
 
-// One 128 x 128 tile per block.  Thread (g, c) holds rows 8 g .. 8 g + 7 and
+// One 128 x 128 tile per block.  Thread (g, c) holds rows 4 g .. 4 g + 3 and
 // columns 8 c .. 8 c + 7: a row of the tile is 16 lanes' 16-byte loads, and
-// the thread's 8 rows of one column are 8 consecutive bytes of the turned
-// tile, which goes out through shared memory.
+// the thread's 4 rows of one column are 4 consecutive bytes of the turned
+// tile, which goes out through shared memory.  32 elements a thread keep it
+// at 64 registers, so that two blocks of 16 warps hide each other's loads.
 template <typename T, bool VEC, int BLOCK_ROWS, bool NORMAL, bool TURNED>
 __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams P) {
-    __shared__ __align__(16) unsigned char tile[TURNED ? kTile * kTile : 16];
-    __shared__ uint32_t tops[TURNED && BLOCK_ROWS == 1 ? 8 : 1][kTile];
-    __shared__ uint32_t top_all[8];
-    const uint32_t g = threadIdx.x >> 4, c = threadIdx.x & 15, warp = threadIdx.x >> 5;
+    constexpr int kWarps = kThreads / 32;
+    __shared__ __align__(16) uint32_t tile[TURNED ? kTile * kTile / 4 : 4];
+    __shared__ __align__(16) float tops[TURNED && BLOCK_ROWS == 1 ? kWarps : 1][kTile];
+    __shared__ __align__(16) float inverses[TURNED && BLOCK_ROWS == 1 ? kTile : 4];
+    __shared__ float top_all[kWarps];
+    const uint32_t g = threadIdx.x >> 4, c = threadIdx.x & 15, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t kb = blockIdx.x % P.k_blocks, mb = blockIdx.x / P.k_blocks;
     const uint32_t row0 = mb * kTile + g * kRows, col0 = kb * kTile + c * 8;
     const int left = int(P.k) - int(col0);
@@ -116,23 +112,84 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
             for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
         }
     }
-
-    uint32_t whole = 127;  // scale exponent of the 128 x 128 block
-    if (BLOCK_ROWS == 128) {
-        uint32_t top = 0;
+    if (TURNED && P.sums) {
+        // column sums of the tile, rows in a fixed order
+        float sum[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sum[i] = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+        }
+        float *sums = reinterpret_cast<float *>(tile);  // [kWarps][kTile]
+        if (lane < 16) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4 *>(sums + warp * kTile + c * 8 + i) =
+                    make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+        }
+        __syncthreads();
+        if (threadIdx.x < kTile && kb * kTile + threadIdx.x < P.k) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) s += sums[w * kTile + threadIdx.x];
+            P.sums[size_t(mb) * P.k + kb * kTile + threadIdx.x] = s;
+        }
+        __syncthreads();
+    }
+    // infinities become NaN, which the maxima below pass over (0 * v is 0
+    // for every finite v, so most threads find none)
+    float any = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) any = fmaf(v[r][i], 0.0f, any);
+    if (any != 0.0f) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[r][i]));
-        top = __reduce_max_sync(0xffffffffu, top);
-        if ((threadIdx.x & 31) == 0) top_all[warp] = top;
+            for (int i = 0; i < 8; ++i)
+                if (fabsf(v[r][i]) == __int_as_float(0x7f800000)) v[r][i] = __int_as_float(0x7fc00000);
+    }
+
+    uint32_t whole = 127;  // scale exponent of the 128 x 128 block
+    if (BLOCK_ROWS == 128) {
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[r][i]));
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        if (lane == 0) top_all[warp] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) top = max(top, top_all[w]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, top_all[w]);
         whole = scale_exponent(top);
         if (threadIdx.x == 0) {
             if (NORMAL) P.scales[size_t(kb) * P.m_blocks + mb] = scale_value(whole);
             if (TURNED) P.turned_scales[size_t(mb) * P.k_blocks + kb] = scale_value(whole);
+        }
+    }
+    if (TURNED && BLOCK_ROWS == 1) {
+        float top[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            top[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
+            top[i] = fmaxf(0.0f, top[i]);  // four NaN
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+        }
+        if (lane < 16) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4 *>(&tops[warp][c * 8 + i]) = make_float4(top[i], top[i + 1], top[i + 2], top[i + 3]);
+        }
+        __syncthreads();
+        if (threadIdx.x < kTile) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) t = fmaxf(t, tops[w][threadIdx.x]);
+            const uint32_t e = scale_exponent(t), col = kb * kTile + threadIdx.x;
+            inverses[threadIdx.x] = scale_inverse(e);
+            if (col < P.k) P.turned_scales[size_t(mb) * P.k + col] = scale_value(e);
         }
     }
 
@@ -141,11 +198,11 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
         for (int r = 0; r < kRows; ++r) {
             uint32_t exponent = whole;
             if (BLOCK_ROWS == 1) {
-                uint32_t top = 0;
+                float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[r][i]));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[r][i]));
 #pragma unroll
-                for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 exponent = scale_exponent(top);
             }
             const float inv = scale_inverse(exponent);
@@ -154,8 +211,8 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
                 // whole 16-byte pieces of the row are written, zeros past k
                 if (col0 < ((P.k + 15u) & ~15u)) {
                     uint2 q;
-                    q.x = pack4(scaled(v[r][0], inv), scaled(v[r][1], inv), scaled(v[r][2], inv), scaled(v[r][3], inv));
-                    q.y = pack4(scaled(v[r][4], inv), scaled(v[r][5], inv), scaled(v[r][6], inv), scaled(v[r][7], inv));
+                    q.x = pack4(v[r][0] * inv, v[r][1] * inv, v[r][2] * inv, v[r][3] * inv);
+                    q.y = pack4(v[r][4] * inv, v[r][5] * inv, v[r][6] * inv, v[r][7] * inv);
                     *reinterpret_cast<uint2 *>(P.values + size_t(row0 + r) * P.ldv + col0) = q;
                 }
             }
@@ -163,58 +220,71 @@ __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams
     }
 
     if (TURNED) {
-        uint32_t exponent[8];
+        float inv[8];
         if (BLOCK_ROWS == 1) {
-            uint32_t top[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                top[i] = 0;
-#pragma unroll
-                for (int r = 0; r < kRows; ++r) top[i] = max(top[i], magnitude(v[r][i]));
-                top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-            }
-            if ((threadIdx.x & 31) < 16) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) tops[warp][c * 8 + i] = top[i];
-            }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-#pragma unroll
-                for (int w = 0; w < 8; ++w) top[i] = max(top[i], tops[w][c * 8 + i]);
-                exponent[i] = scale_exponent(top[i]);
-            }
-            if (g == 0) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < left) P.turned_scales[size_t(mb) * P.k + col0 + i] = scale_value(exponent[i]);
+            for (int i = 0; i < 8; i += 4) {
+                const float4 q = *reinterpret_cast<const float4 *>(&inverses[c * 8 + i]);
+                inv[i] = q.x;
+                inv[i + 1] = q.y;
+                inv[i + 2] = q.z;
+                inv[i + 3] = q.w;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) exponent[i] = whole;
+            for (int i = 0; i < 8; ++i) inv[i] = scale_inverse(whole);
         }
-        // column j of the tile: 16 pieces of 8 rows, piece g at place
-        // g ^ (j / 8), so that the lanes of a store fall on different banks
+        // column j of the tile: 32 words of 4 rows, word g at place
+        // g ^ 2 (j / 8), so that the lanes of a store fall on different banks
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float inv = scale_inverse(exponent[i]);
-            uint2 q;
-            q.x = pack4(scaled(v[0][i], inv), scaled(v[1][i], inv), scaled(v[2][i], inv), scaled(v[3][i], inv));
-            q.y = pack4(scaled(v[4][i], inv), scaled(v[5][i], inv), scaled(v[6][i], inv), scaled(v[7][i], inv));
-            *reinterpret_cast<uint2 *>(tile + (c * 8 + i) * kTile + ((g ^ c) << 3)) = q;
-        }
+        for (int i = 0; i < 8; ++i)
+            tile[(c * 8 + i) * 32 + (g ^ (2 * c))] = pack4(v[0][i] * inv[i], v[1][i] * inv[i], v[2][i] * inv[i], v[3][i] * inv[i]);
         __syncthreads();
-        // 16 bytes (two pieces) per thread and turn: whole 16-byte pieces of
-        // the turned rows, zeros past m
+        // 16 bytes per thread and turn: whole 16-byte pieces of the turned
+        // rows, zeros past m
         const uint32_t m16 = (P.m + 15u) & ~15u;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < int(kTile * 8 / kThreads); ++t) {
             const uint32_t at = t * kThreads + threadIdx.x, j = at >> 3, s = at & 7, turn = (j >> 3) & 15;
-            uint4 q = *reinterpret_cast<const uint4 *>(tile + j * kTile + (((2 * s) ^ (turn & ~1u)) << 3));
+            uint4 q = *reinterpret_cast<const uint4 *>(tile + j * 32 + ((s ^ (turn >> 1)) << 2));
             if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
             const uint32_t row = kb * kTile + j, col = mb * kTile + 16 * s;
             if (row < P.k && col < m16) *reinterpret_cast<uint4 *>(P.turned + size_t(row) * P.ldt + col) = q;
         }
+    }
+}
+
+// out[c] = the sums of 128 rows, added up in order.
+template <typename T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 32 columns per block, 32 runs of consecutive rows each; the runs' sums are
+// added in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) add_sums_kernel(const float *__restrict__ sums, uint32_t rows, uint32_t k,
+                                                        T *__restrict__ out) {
+    __shared__ float part[32][33];
+    const uint32_t x = threadIdx.x & 31, y = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
+    const uint32_t per = (rows + 31) / 32, beg = min(rows, y * per), end = min(rows, beg + per);
+    float s = 0.0f;
+    if (col < k) {
+#pragma unroll 8
+        for (uint32_t r = beg; r < end; ++r) s += sums[size_t(r) * k + col];
+    }
+    part[y][x] = s;
+    __syncthreads();
+    if (y == 0 && col < k) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t += part[i][x];
+        out[col] = round_to<T>(t);
     }
 }
 
@@ -246,21 +316,21 @@ __device__ __forceinline__ float e4m3_float(uint32_t byte) {
     return __half2float(__half(h));
 }
 
-constexpr int kDequantItems = 4;
+constexpr int kDequantThreads = 256, kDequantItems = 4;
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const unsigned char *__restrict__ values, size_t ldv,
+__global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(const unsigned char *__restrict__ values, size_t ldv,
                                                               const float *__restrict__ scales, uint32_t shift,
                                                               size_t scale_row, size_t scale_block, uint32_t m,
                                                               uint32_t k, uint32_t units,
                                                               T *__restrict__ out) {
     const uint64_t total = uint64_t(m) * units;
-    const uint64_t first = uint64_t(blockIdx.x) * (kThreads * kDequantItems);
+    const uint64_t first = uint64_t(blockIdx.x) * (kDequantThreads * kDequantItems);
     const uint64_t row0 = first / units;
     const uint32_t col0 = uint32_t(first - row0 * units);
 #pragma unroll
     for (int t = 0; t < kDequantItems; ++t) {
-        const uint32_t e = t * kThreads + threadIdx.x;
+        const uint32_t e = t * kDequantThreads + threadIdx.x;
         if (first + e >= total) return;
         const uint32_t r = (col0 + e) / units, u = (col0 + e) - r * units, col = u * VEC;
         const uint64_t row = row0 + r;
@@ -301,18 +371,19 @@ void dequantize_typed(const void *values, size_t ldv, const float *scales, size_
     const bool vec = k % 4 == 0 && ldv % 4 == 0 && (reinterpret_cast<uintptr_t>(values) & 3u) == 0 &&
                      (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
     const uint32_t units = vec ? k / 4 : k, shift = block_rows == 128 ? 7 : 0;
-    const uint64_t per = kThreads * kDequantItems;
+    const uint64_t per = kDequantThreads * kDequantItems;
     const unsigned blocks = unsigned((uint64_t(m) * units + per - 1) / per);
     const unsigned char *v = static_cast<const unsigned char *>(values);
-    if (vec) dequantize_kernel<T, 4><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
-    else dequantize_kernel<T, 1><<<blocks, kThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
+    if (vec) dequantize_kernel<T, 4><<<blocks, kDequantThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
+    else dequantize_kernel<T, 1><<<blocks, kDequantThreads, 0, stream>>>(v, ldv, scales, shift, scale_row, scale_block, m, k, units, static_cast<T *>(out));
 }
 
 }  // namespace
 
 cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint32_t m, uint32_t k, int block_rows,
                                   void *values, size_t ldv, float *scales, void *turned, size_t ldt,
-                                  float *turned_scales, cudaStream_t stream) {
+                                  float *turned_scales, float *sums, void *column_sums, uint32_t sums_dtype,
+                                  cudaStream_t stream) {
     if (m == 0 || k == 0) return cudaSuccess;
     QuantParams P{};
     P.x = x;
@@ -325,6 +396,7 @@ cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint
     P.ldt = ldt;
     P.scales = scales;
     P.turned_scales = turned_scales;
+    P.sums = column_sums ? sums : nullptr;
     P.k_blocks = (k + kTile - 1) / kTile;
     P.m_blocks = (m + kTile - 1) / kTile;
     const unsigned blocks = P.k_blocks * P.m_blocks;
@@ -332,6 +404,14 @@ cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint
         case SDFOAM_F32: quantize_typed<float>(P, block_rows, blocks, stream); break;
         case SDFOAM_F16: quantize_typed<__half>(P, block_rows, blocks, stream); break;
         default: quantize_typed<__nv_bfloat16>(P, block_rows, blocks, stream); break;
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || !column_sums) return e;
+    const unsigned columns = (k + 31) / 32;
+    switch (sums_dtype) {
+        case SDFOAM_F32: add_sums_kernel<<<columns, 1024, 0, stream>>>(sums, P.m_blocks, k, static_cast<float *>(column_sums)); break;
+        case SDFOAM_F16: add_sums_kernel<<<columns, 1024, 0, stream>>>(sums, P.m_blocks, k, static_cast<__half *>(column_sums)); break;
+        default: add_sums_kernel<<<columns, 1024, 0, stream>>>(sums, P.m_blocks, k, static_cast<__nv_bfloat16 *>(column_sums)); break;
     }
     return cudaGetLastError();
 }

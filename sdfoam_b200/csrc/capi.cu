@@ -664,7 +664,8 @@ int sdfoam_lookup_rows_backward(const void *grad, uint32_t columns, uint64_t ld,
 
 int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m, uint64_t k, int block_rows,
                           void *values, uint64_t ldv, float *scales, void *turned, uint64_t ldt,
-                          float *turned_scales, sdfoam_stream_t stream) {
+                          float *turned_scales, void *column_sums, uint32_t sums_dtype, float *workspace,
+                          sdfoam_stream_t stream) {
     int rc = check_blocks(m, k, block_rows);
     if (rc != SDFOAM_OK) return rc;
     if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
@@ -675,10 +676,12 @@ int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m
         if (!aligned_to(x, dtype)) return fail(SDFOAM_ERR_INVALID, "x must be aligned to its elements");
         if ((values && (ldv % 16 || ldv < k || !aligned16(values))) || (turned && (ldt % 16 || ldt < m || !aligned16(turned))))
             return fail(SDFOAM_ERR_INVALID, "rows of values must be multiples of 16 bytes and 16-byte aligned");
+        if (column_sums && (!turned || !workspace || sums_dtype > SDFOAM_BF16 || !aligned_to(column_sums, sums_dtype)))
+            return fail(SDFOAM_ERR_INVALID, "column_sums need turned, a workspace and a type");
     }
     cudaError_t e = launch_block_quantize(x, ld, dtype, static_cast<uint32_t>(m), static_cast<uint32_t>(k), block_rows,
-                                          values, ldv, scales, turned, ldt, turned_scales,
-                                          reinterpret_cast<cudaStream_t>(stream));
+                                          values, ldv, scales, turned, ldt, turned_scales, workspace, column_sums,
+                                          sums_dtype, reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_quantize");
 }
 

@@ -101,7 +101,8 @@ cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t co
 // the product of two such matrices (block_mm.cu).
 cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint32_t m, uint32_t k, int block_rows,
                                   void *values, size_t ldv, float *scales, void *turned, size_t ldt,
-                                  float *turned_scales, cudaStream_t stream);
+                                  float *turned_scales, float *sums, void *column_sums, uint32_t sums_dtype,
+                                  cudaStream_t stream);
 cudaError_t launch_block_dequantize(const void *values, size_t ldv, const float *scales, size_t scale_row,
                                     size_t scale_block, int block_rows, uint32_t m, uint32_t k, uint32_t dtype,
                                     void *out, cudaStream_t stream);

@@ -393,8 +393,9 @@ def test_entry_points_refuse_bad_arguments():
     def message():
         return lib.sdfoam_last_error().decode()
 
-    def quantize(x=p, ld=32, dtype=0, m=4, k=32, rows=1, v=p, ldv=32, s=p, t=None, ldt=0, ts=None):
-        return lib.sdfoam_block_quantize(x, ld, dtype, m, k, rows, v, ldv, s, t, ldt, ts, None)
+    def quantize(x=p, ld=32, dtype=0, m=4, k=32, rows=1, v=p, ldv=32, s=p, t=None, ldt=0, ts=None, sums=None, st=0,
+                 ws=None):
+        return lib.sdfoam_block_quantize(x, ld, dtype, m, k, rows, v, ldv, s, t, ldt, ts, sums, st, ws, None)
 
     assert quantize(rows=2) == 1 and "block_rows" in message()
     assert quantize(dtype=3) == 2
@@ -404,6 +405,8 @@ def test_entry_points_refuse_bad_arguments():
     assert quantize(v=None) == 1 and quantize(s=None) == 1 and quantize(x=None) == 1
     assert quantize(ldv=40) == 1 and quantize(ldv=16) == 1 and quantize(v=ctypes.c_void_p(4100)) == 1
     assert quantize(t=p, ldt=8, ts=p) == 1 and quantize(t=p, ldt=16) == 1
+    assert quantize(sums=p, ws=p) == 1 and "column_sums" in message()
+    assert quantize(t=p, ldt=16, ts=p, sums=p) == 1 and quantize(t=p, ldt=16, ts=p, sums=p, ws=p, st=3) == 1
     assert quantize(m=0, x=None, v=None) == 0
 
     def dequantize(v=p, ldv=32, s=p, rows=1, m=4, k=32, dtype=0, out=p):
