@@ -519,6 +519,30 @@ SDFOAM_API int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_s
                                    uint32_t out_dtype, void *workspace, size_t workspace_bytes, int *error,
                                    sdfoam_stream_t stream);
 
+/* A linear layer of such products, y = Q(x) Q(weight)^T + bias, for training:
+ * x [m, k], weight [n, k], y [m, n] contiguous of x's type; Q quantizes in
+ * blocks of 1 x 128 (x, dy and their transposes) and 128 x 128 (weight).
+ *   forward: keeps x (keep_x) and the weight (keep_weight) turned in `saved`
+ *     for the backward.
+ *   backward: dx = Q(dy) Q(weight) [m, k], dweight = Q(dy^T) Q(x^T)^T [n, k],
+ *     dbias = sum dy [n], each contiguous and optional (NULL); kept_x and
+ *     kept_weight as in the forward.
+ * saved and workspace are sized by the two queries (the workspace serves
+ * either call, and calls on one stream may share it), 16-byte aligned. */
+SDFOAM_API size_t sdfoam_block_linear_saved_bytes(uint64_t m, uint64_t n, uint64_t k, int with_x, int with_weight);
+SDFOAM_API size_t sdfoam_block_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k);
+SDFOAM_API int sdfoam_block_linear_forward(const void *x, uint64_t ldx, uint32_t x_dtype, uint64_t m,
+                                           const void *weight, uint64_t ldw, uint32_t weight_dtype, uint64_t n,
+                                           uint64_t k, const void *bias, uint32_t bias_dtype, void *y, void *saved,
+                                           size_t saved_bytes, int keep_x, int keep_weight, void *workspace,
+                                           size_t workspace_bytes, int *error, sdfoam_stream_t stream);
+SDFOAM_API int sdfoam_block_linear_backward(const void *dy, uint64_t ldy, uint32_t dy_dtype, uint64_t m, uint64_t n,
+                                            uint64_t k, const void *saved, size_t saved_bytes, int kept_x,
+                                            int kept_weight, void *dx, uint32_t dx_dtype, void *dweight,
+                                            uint32_t dweight_dtype, void *dbias, uint32_t dbias_dtype,
+                                            void *workspace, size_t workspace_bytes, int *error,
+                                            sdfoam_stream_t stream);
+
 /* Allocation-free sdfoam_trace_forward.  No counterpart in the reference: it
  * exists for callers that cannot allocate device memory -- hosts reaching this
  * library through the C ABI without a device allocator of their own, and frame

@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 # SDFOAM_B200_LIB selects another build of the same library (same ABI).
 LIB_PATH = os.environ.get("SDFOAM_B200_LIB") or os.path.join(HERE, "libsdfoam_b200.so")
@@ -68,6 +70,10 @@ EXPORTED = (
     "sdfoam_block_dequantize",
     "sdfoam_block_matmul_workspace_bytes",
     "sdfoam_block_matmul",
+    "sdfoam_block_linear_saved_bytes",
+    "sdfoam_block_linear_workspace_bytes",
+    "sdfoam_block_linear_forward",
+    "sdfoam_block_linear_backward",
 )
 
 
@@ -265,6 +271,17 @@ def load():
     lib.sdfoam_block_matmul.restype = ctypes.c_int
     lib.sdfoam_block_matmul.argtypes = [vp, u64, vp, u64, u64, i32, u64, vp, u64, vp, u64, u64, i32, u64, u64, vp, u32,
                                         vp, u64, u32, vp, ctypes.c_size_t, vp, vp]
+    size = ctypes.c_size_t
+    lib.sdfoam_block_linear_saved_bytes.restype = size
+    lib.sdfoam_block_linear_saved_bytes.argtypes = [u64, u64, u64, i32, i32]
+    lib.sdfoam_block_linear_workspace_bytes.restype = size
+    lib.sdfoam_block_linear_workspace_bytes.argtypes = [u64, u64, u64]
+    lib.sdfoam_block_linear_forward.restype = ctypes.c_int
+    lib.sdfoam_block_linear_forward.argtypes = [vp, u64, u32, u64, vp, u64, u32, u64, u64, vp, u32, vp, vp, size, i32,
+                                                i32, vp, size, vp, vp]
+    lib.sdfoam_block_linear_backward.restype = ctypes.c_int
+    lib.sdfoam_block_linear_backward.argtypes = [vp, u64, u32, u64, u64, u64, vp, size, i32, i32, vp, u32, vp, u32, vp,
+                                                 u32, vp, size, vp, vp]
     _lib = lib
     return lib
 
@@ -273,3 +290,27 @@ def check(rc: int) -> None:
     if rc != SDFOAM_OK:
         msg = load().sdfoam_last_error().decode("utf-8", "replace")
         raise RuntimeError(msg)
+
+
+class _Same:
+    """The current device is the right one already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME = _Same()
+
+
+def on(device: torch.device):
+    """A context in which `device` is the current CUDA device."""
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream(device: torch.device) -> int:
+    """The handle of the device's current stream (without a Stream object:
+    a call of these operators takes microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)

@@ -39,21 +39,23 @@ def _matrix(x: torch.Tensor) -> torch.Tensor:
 
 
 # One word per device in pinned host memory, which a kernel that gives up
-# waiting writes and the host reads without a copy.
+# waiting writes and the host reads without a copy: (tensor, its numpy view,
+# its address).
 _flags: dict = {}
 
 
-def _flag(device: torch.device) -> torch.Tensor:
+def _flag(device: torch.device) -> int:
     f = _flags.get(device.index)
     if f is None:
-        f = _flags[device.index] = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-    elif f[0]:
+        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        f = _flags[device.index] = (t, t.numpy(), t.data_ptr())
+    elif f[1][0]:
         _raise(f)
-    return f
+    return f[2]
 
 
 def _raise(f):
-    f.zero_()
+    f[1][0] = 0
     raise RuntimeError("an 8-bit product gave up waiting on the tensor-core pipeline and wrote NaN")
 
 
@@ -63,7 +65,7 @@ def check_block_flags():
     (the next product on the device raises it too)."""
     for index, f in _flags.items():
         torch.cuda.synchronize(index)
-        if f[0]:
+        if f[1][0]:
             _raise(f)
 
 
@@ -74,34 +76,21 @@ def _values(rows: int, columns: int, device) -> torch.Tensor:
     return v if ld == columns else v[:, :columns]
 
 
-def _quantize(x, block_rows, normal, turned, sums=None):
-    """(values, scales) or None of x and of x turned; the sums of x's columns
-    go to the vector ``sums`` (only with turned)."""
+def _quantize(x, block_rows, turned):
+    """(values, scales) of x, or of x turned."""
     x = _matrix(x)
     m, k = x.shape
     dev = x.device
-    v = s = vt = st = None
-    if normal:
-        v = _values(m, k, dev)
-        s = torch.empty((_blocks(k), m if block_rows == 1 else _blocks(m)), dtype=torch.float32, device=dev).t()
-    if turned:
-        vt = _values(k, m, dev)
-        st = torch.empty((_blocks(m), k if block_rows == 1 else _blocks(k)), dtype=torch.float32, device=dev).t()
-    ws = None
-    if sums is not None:
-        if m == 0:
-            sums.zero_()
-        ws = torch.empty((_blocks(m), k), dtype=torch.float32, device=dev)
+    rows, columns = (k, m) if turned else (m, k)
+    v = _values(rows, columns, dev)
+    s = torch.empty((_blocks(columns), rows if block_rows == 1 else _blocks(rows)), dtype=torch.float32, device=dev)
+    at = (v.data_ptr(), max(v.stride(0), columns), s.data_ptr())
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        _lib.check(lib.sdfoam_block_quantize(
-            x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, k, block_rows,
-            v.data_ptr() if normal else None, max(v.stride(0), k) if normal else 0, s.data_ptr() if normal else None,
-            vt.data_ptr() if turned else None, max(vt.stride(0), m) if turned else 0,
-            st.data_ptr() if turned else None, None if sums is None else sums.data_ptr(),
-            0 if sums is None else _DTYPES[sums.dtype], None if ws is None else ws.data_ptr(),
-            torch.cuda.current_stream().cuda_stream))
-    return (v, s) if normal else None, (vt, st) if turned else None
+    with _lib.on(dev):
+        _lib.check(lib.sdfoam_block_quantize(x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, k, block_rows,
+                                             *((None, 0, None, *at) if turned else (*at, None, 0, None)), None, 0,
+                                             None, _lib.stream(dev)))
+    return v, s.t()
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int = 1, transpose: bool = False):
@@ -122,7 +111,7 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1, transpose: bool = Fals
     if block_rows not in (1, _BLOCK):
         raise RuntimeError("block_rows must be 1 or 128")
     _cuda("x", x)
-    return _quantize(x.detach(), block_rows, not transpose, bool(transpose))[int(bool(transpose))]
+    return _quantize(x.detach(), block_rows, bool(transpose))
 
 
 def _block_rows(what: str, values: torch.Tensor, scales: torch.Tensor) -> int:
@@ -152,10 +141,10 @@ def dequantize_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.d
     m, k = v.shape
     out = torch.empty((m, k), dtype=dtype, device=v.device)
     lib = _lib.load()
-    with torch.cuda.device(v.device):
+    with _lib.on(v.device):
         _lib.check(lib.sdfoam_block_dequantize(v.data_ptr(), max(v.stride(0), k), s.data_ptr(), s.stride(0), s.stride(1),
                                                block_rows, m, k, _DTYPES[dtype], out.data_ptr(),
-                                               torch.cuda.current_stream().cuda_stream))
+                                               _lib.stream(v.device)))
     return out
 
 
@@ -177,15 +166,14 @@ def _product(a, a_scales, a_rows, b, b_scales, b_rows, bias, out_dtype):
     out = torch.empty((m, n), dtype=out_dtype, device=dev)
     lib = _lib.load()
     nbytes = lib.sdfoam_block_matmul_workspace_bytes(m, n, k)
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         _lib.check(lib.sdfoam_block_matmul(
             a.data_ptr(), max(a.stride(0), k), a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), a_rows, m,
             b.data_ptr(), max(b.stride(0), k), b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), b_rows,
             n, k, None if bias is None else bias.data_ptr(),
             0 if bias is None else _DTYPES[bias.dtype], out.data_ptr(), max(n, 1), _DTYPES[out_dtype],
-            None if ws is None else ws.data_ptr(), nbytes, _flag(dev).data_ptr(),
-            torch.cuda.current_stream().cuda_stream))
+            None if ws is None else ws.data_ptr(), nbytes, _flag(dev), _lib.stream(dev)))
     return out
 
 
@@ -220,29 +208,53 @@ def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        # one pass over each operand writes it in rows and, for the gradient
-        # that reduces along the other axis, turned
-        q, qt = _quantize(x, 1, True, need_w)
-        w, wt = _quantize(weight, _BLOCK, True, need_x)
-        ctx.save_for_backward(*(qt or (None, None)), *(wt or (None, None)))
+        # x is kept (turned, in 8 bits) for the weight's gradient and the
+        # weight for x's
+        keep_w, keep_x = ctx.needs_input_grad[:2]
+        x, weight = _matrix(x), _matrix(weight)
+        m, k = x.shape
+        n = weight.shape[0]
+        dev = x.device
+        lib = _lib.load()
+        y = torch.empty((m, n), dtype=x.dtype, device=dev)
+        saved_bytes = lib.sdfoam_block_linear_saved_bytes(m, n, k, keep_x, keep_w)
+        saved = torch.empty((saved_bytes,), dtype=torch.uint8, device=dev)
+        nbytes = lib.sdfoam_block_linear_workspace_bytes(m, n, k)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        if bias is not None:
+            bias = bias.contiguous()
+        with _lib.on(dev):
+            _lib.check(lib.sdfoam_block_linear_forward(
+                x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, weight.data_ptr(), max(weight.stride(0), k),
+                _DTYPES[weight.dtype], n, k, None if bias is None else bias.data_ptr(),
+                0 if bias is None else _DTYPES[bias.dtype], y.data_ptr(), saved.data_ptr(), saved_bytes, keep_x, keep_w,
+                ws.data_ptr(), nbytes, _flag(dev), _lib.stream(dev)))
+        ctx.save_for_backward(saved)
+        ctx.kept = keep_x, keep_w
+        ctx.sizes = m, n, k
         ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
-        return _product(*q, 1, *w, _BLOCK, None if bias is None else bias.contiguous(), x.dtype)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        qt, qts, wt, wts = ctx.saved_tensors
+        (saved,) = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
-        dx = dw = db = None
-        if need_b:
-            db = torch.empty((grad.shape[1],), dtype=ctx.dtypes[2], device=grad.device)
-        # one pass over dy: its values for both products and its column sums
-        g, gt = _quantize(grad, 1, need_x, need_w or need_b, db)
-        if need_x:
-            dx = _product(*g, 1, wt, wts, _BLOCK, None, ctx.dtypes[0])
-        if need_w:
-            dw = _product(*gt, 1, qt, qts, 1, None, ctx.dtypes[1])
+        m, n, k = ctx.sizes
+        grad = _matrix(grad)
+        dev = grad.device
+        lib = _lib.load()
+        dx = torch.empty((m, k), dtype=ctx.dtypes[0], device=dev) if need_x else None
+        dw = torch.empty((n, k), dtype=ctx.dtypes[1], device=dev) if need_w else None
+        db = torch.empty((n,), dtype=ctx.dtypes[2], device=dev) if need_b else None
+        nbytes = lib.sdfoam_block_linear_workspace_bytes(m, n, k)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        with _lib.on(dev):
+            _lib.check(lib.sdfoam_block_linear_backward(
+                grad.data_ptr(), max(grad.stride(0), n), _DTYPES[grad.dtype], m, n, k, saved.data_ptr(),
+                saved.numel(), *ctx.kept, None if dx is None else dx.data_ptr(), _DTYPES[ctx.dtypes[0]],
+                None if dw is None else dw.data_ptr(), _DTYPES[ctx.dtypes[1]], None if db is None else db.data_ptr(),
+                0 if db is None else _DTYPES[db.dtype], ws.data_ptr(), nbytes, _flag(dev), _lib.stream(dev)))
         return dx, dw, db
 
 

@@ -50,6 +50,61 @@ int check_blocks(uint64_t m, uint64_t k, int block_rows) {
     return SDFOAM_OK;
 }
 
+// A linear layer of 8-bit products: every matrix of it and of its gradients.
+int check_layer(uint64_t m, uint64_t n, uint64_t k) {
+    int rc = check_blocks(m, n, 1);
+    if (rc == SDFOAM_OK) rc = check_blocks(m, k, 1);
+    return rc == SDFOAM_OK ? check_blocks(n, k, 1) : rc;
+}
+
+// Its buffers: what the forward keeps for the backward (x and the weight
+// turned, values and scales), and the workspaces of either.
+struct LayerLayout {
+    uint64_t ldm, ldn, ldk;      // 16-byte rows over m, n, k
+    uint64_t nb, kb;             // blocks of 128 of n, k
+    size_t xt, xts, wt, wts, saved;
+    size_t xq, xs, wq, wsc, parts_forward, forward;
+    size_t gq, gs, gt, gts, sums, parts_backward, backward;
+
+    static LayerLayout make(uint64_t m, uint64_t n, uint64_t k, bool with_x, bool with_weight) {
+        LayerLayout l{};
+        l.ldm = align_up(m, 16);
+        l.ldn = align_up(n, 16);
+        l.ldk = align_up(k, 16);
+        const uint64_t mb = (m + 127) / 128;
+        l.nb = (n + 127) / 128;
+        l.kb = (k + 127) / 128;
+        size_t at = 0;
+        auto take = [&at](size_t bytes) {
+            const size_t here = at;
+            at += align_up(bytes, 256);
+            return here;
+        };
+        l.xt = take(with_x ? k * l.ldm : 0);
+        l.xts = take(with_x ? mb * k * 4 : 0);
+        l.wt = take(with_weight ? k * l.ldn : 0);
+        l.wts = take(with_weight ? l.nb * l.kb * 4 : 0);
+        l.saved = at;
+        at = 0;
+        l.xq = take(m * l.ldk);
+        l.xs = take(l.kb * m * 4);
+        l.wq = take(n * l.ldk);
+        l.wsc = take(l.nb * l.kb * 4);
+        l.parts_forward = at;
+        l.forward = at + sdfoam_block_matmul_workspace_bytes(m, n, k);
+        at = 0;
+        l.gq = take(m * l.ldn);
+        l.gs = take(l.nb * m * 4);
+        l.gt = take(n * l.ldm);
+        l.gts = take(mb * n * 4);
+        l.sums = take(mb * n * 4);
+        l.parts_backward = at;
+        const size_t dx = sdfoam_block_matmul_workspace_bytes(m, k, n), dw = sdfoam_block_matmul_workspace_bytes(n, k, m);
+        l.backward = at + (dx > dw ? dx : dw);
+        return l;
+    }
+};
+
 // sdfoam_lookup_rows and its gradient.
 int check_lookup(uint32_t dtype, uint32_t id_type, uint32_t columns, uint64_t ld) {
     if (dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported table type");
@@ -679,6 +734,11 @@ int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m
         if (column_sums && (!turned || !workspace || sums_dtype > SDFOAM_BF16 || !aligned_to(column_sums, sums_dtype)))
             return fail(SDFOAM_ERR_INVALID, "column_sums need turned, a workspace and a type");
     }
+    if (m == 0 && k > 0 && column_sums) {
+        cudaError_t z = cudaMemsetAsync(column_sums, 0, k * (sums_dtype == SDFOAM_F32 ? 4 : 2),
+                                        reinterpret_cast<cudaStream_t>(stream));
+        return z == cudaSuccess ? SDFOAM_OK : cuda_fail(z, "sdfoam_block_quantize");
+    }
     cudaError_t e = launch_block_quantize(x, ld, dtype, static_cast<uint32_t>(m), static_cast<uint32_t>(k), block_rows,
                                           values, ldv, scales, turned, ldt, turned_scales, workspace, column_sums,
                                           sums_dtype, reinterpret_cast<cudaStream_t>(stream));
@@ -735,6 +795,84 @@ int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint
                                         bias_dtype, out, ldo, out_dtype, workspace, error,
                                         reinterpret_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SDFOAM_OK : cuda_fail(e, "sdfoam_block_matmul");
+}
+
+size_t sdfoam_block_linear_saved_bytes(uint64_t m, uint64_t n, uint64_t k, int with_x, int with_weight) {
+    if (check_layer(m, n, k) != SDFOAM_OK) return 0;
+    return LayerLayout::make(m, n, k, with_x != 0, with_weight != 0).saved;
+}
+
+size_t sdfoam_block_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k) {
+    if (check_layer(m, n, k) != SDFOAM_OK) return 0;
+    const LayerLayout l = LayerLayout::make(m, n, k, true, true);
+    return l.forward > l.backward ? l.forward : l.backward;
+}
+
+int sdfoam_block_linear_forward(const void *x, uint64_t ldx, uint32_t x_dtype, uint64_t m, const void *weight,
+                                uint64_t ldw, uint32_t weight_dtype, uint64_t n, uint64_t k, const void *bias,
+                                uint32_t bias_dtype, void *y, void *saved, size_t saved_bytes, int keep_x,
+                                int keep_weight, void *workspace, size_t workspace_bytes, int *error,
+                                sdfoam_stream_t stream) {
+    int rc = check_layer(m, n, k);
+    if (rc != SDFOAM_OK) return rc;
+    if (x_dtype > SDFOAM_BF16 || weight_dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
+    const LayerLayout l = LayerLayout::make(m, n, k, keep_x != 0, keep_weight != 0);
+    if ((l.saved > 0 && (!saved || saved_bytes < l.saved || !aligned16(saved))) ||
+        (l.forward > 0 && (!workspace || workspace_bytes < l.forward || !aligned16(workspace))))
+        return fail(SDFOAM_ERR_INVALID, "saved or workspace is too small or not 16-byte aligned");
+    char *sv = static_cast<char *>(saved), *ws = static_cast<char *>(workspace);
+    // one pass over each operand: in rows, and turned for the backward
+    rc = sdfoam_block_quantize(x, ldx, x_dtype, m, k, 1, ws + l.xq, l.ldk, reinterpret_cast<float *>(ws + l.xs),
+                               keep_x ? sv + l.xt : nullptr, l.ldm,
+                               keep_x ? reinterpret_cast<float *>(sv + l.xts) : nullptr, nullptr, 0, nullptr, stream);
+    if (rc != SDFOAM_OK) return rc;
+    rc = sdfoam_block_quantize(weight, ldw, weight_dtype, n, k, 128, ws + l.wq, l.ldk,
+                               reinterpret_cast<float *>(ws + l.wsc), keep_weight ? sv + l.wt : nullptr, l.ldn,
+                               keep_weight ? reinterpret_cast<float *>(sv + l.wts) : nullptr, nullptr, 0, nullptr,
+                               stream);
+    if (rc != SDFOAM_OK) return rc;
+    return sdfoam_block_matmul(ws + l.xq, l.ldk, reinterpret_cast<const float *>(ws + l.xs), 1, m, 1, m, ws + l.wq,
+                               l.ldk, reinterpret_cast<const float *>(ws + l.wsc), 1, l.nb, 128, n, k, bias, bias_dtype,
+                               y, n, x_dtype, ws + l.parts_forward, l.forward - l.parts_forward, error, stream);
+}
+
+int sdfoam_block_linear_backward(const void *dy, uint64_t ldy, uint32_t dy_dtype, uint64_t m, uint64_t n, uint64_t k,
+                                 const void *saved, size_t saved_bytes, int kept_x, int kept_weight, void *dx,
+                                 uint32_t dx_dtype, void *dweight, uint32_t dweight_dtype, void *dbias,
+                                 uint32_t dbias_dtype, void *workspace, size_t workspace_bytes, int *error,
+                                 sdfoam_stream_t stream) {
+    int rc = check_layer(m, n, k);
+    if (rc != SDFOAM_OK) return rc;
+    if ((dx && !kept_weight) || (dweight && !kept_x))
+        return fail(SDFOAM_ERR_INVALID, "dx needs the kept weight and dweight the kept x");
+    if (dy_dtype > SDFOAM_BF16) return fail(SDFOAM_ERR_UNSUPPORTED, "Unsupported matrix type");
+    const LayerLayout l = LayerLayout::make(m, n, k, kept_x != 0, kept_weight != 0);
+    if ((l.saved > 0 && (!saved || saved_bytes < l.saved || !aligned16(saved))) ||
+        (l.backward > 0 && (!workspace || workspace_bytes < l.backward || !aligned16(workspace))))
+        return fail(SDFOAM_ERR_INVALID, "saved or workspace is too small or not 16-byte aligned");
+    const char *sv = static_cast<const char *>(saved);
+    char *ws = static_cast<char *>(workspace);
+    const bool turned = dweight || dbias;
+    if (dx || turned) {
+        // one pass over dy: its values for both products and its column sums
+        rc = sdfoam_block_quantize(dy, ldy, dy_dtype, m, n, 1, dx ? ws + l.gq : nullptr, l.ldn,
+                                   reinterpret_cast<float *>(ws + l.gs), turned ? ws + l.gt : nullptr, l.ldm,
+                                   reinterpret_cast<float *>(ws + l.gts), dbias, dbias_dtype,
+                                   reinterpret_cast<float *>(ws + l.sums), stream);
+        if (rc != SDFOAM_OK) return rc;
+    }
+    if (dx) {
+        rc = sdfoam_block_matmul(ws + l.gq, l.ldn, reinterpret_cast<const float *>(ws + l.gs), 1, m, 1, m, sv + l.wt,
+                                 l.ldn, reinterpret_cast<const float *>(sv + l.wts), 1, l.kb, 128, k, n, nullptr, 0, dx,
+                                 k, dx_dtype, ws + l.parts_backward, l.backward - l.parts_backward, error, stream);
+        if (rc != SDFOAM_OK) return rc;
+    }
+    if (dweight)
+        return sdfoam_block_matmul(ws + l.gt, l.ldm, reinterpret_cast<const float *>(ws + l.gts), 1, n, 1, n,
+                                   sv + l.xt, l.ldm, reinterpret_cast<const float *>(sv + l.xts), 1, k, 1, k, m,
+                                   nullptr, 0, dweight, k, dweight_dtype, ws + l.parts_backward,
+                                   l.backward - l.parts_backward, error, stream);
+    return SDFOAM_OK;
 }
 
 const char *sdfoam_last_error(void) { return g_last_error.c_str(); }

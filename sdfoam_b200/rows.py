@@ -43,10 +43,10 @@ def _lookup(table, ids, scale):
     rows, columns = t.shape
     out = torch.empty((*ids.shape, columns), dtype=t.dtype, device=t.device)
     lib = _lib.load()
-    with torch.cuda.device(t.device):
+    with _lib.on(t.device):
         _lib.check(lib.sdfoam_lookup_rows(t.data_ptr(), rows, columns, max(t.stride(0), columns), _DTYPES[t.dtype],
                                           i.data_ptr(), i.numel(), _ID_TYPES[i.dtype], scale, out.data_ptr(),
-                                          torch.cuda.current_stream().cuda_stream))
+                                          _lib.stream(t.device)))
     return out
 
 
@@ -57,12 +57,12 @@ def _lookup_backward(grad, ids, num_rows, scale):
     out = torch.empty((num_rows, columns), dtype=g.dtype, device=g.device)
     lib = _lib.load()
     nbytes = lib.sdfoam_lookup_rows_workspace_bytes(n, num_rows, columns)
-    with torch.cuda.device(g.device):
+    with _lib.on(g.device):
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=g.device)
         _lib.check(lib.sdfoam_lookup_rows_backward(g.data_ptr(), columns, max(g.stride(0), columns), _DTYPES[g.dtype],
                                                    i.data_ptr(), n, _ID_TYPES[i.dtype], scale, out.data_ptr(),
                                                    num_rows, ws.data_ptr(), nbytes,
-                                                   torch.cuda.current_stream().cuda_stream))
+                                                   _lib.stream(g.device)))
     return out
 
 
@@ -104,6 +104,8 @@ def lookup_rows(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> t
     if table.dim() != 2:
         raise RuntimeError("table must have 2 dimensions")
     _check("table", table, ids)
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return _lookup(table, ids, float(scale))
     return _Lookup.apply(table, ids, float(scale))
 
 
@@ -119,4 +121,6 @@ def lookup_rows_backward(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, s
     if ids.numel() >= 2 ** 31:
         raise RuntimeError("the gradient takes fewer than 2^31 ids")
     _check("grad", grad, ids)
+    if not (grad.requires_grad and torch.is_grad_enabled()):
+        return _lookup_backward(grad, ids, int(num_rows), float(scale))
     return _LookupBackward.apply(grad, ids, int(num_rows), float(scale))
