@@ -79,13 +79,13 @@ struct SortLayout {
 };
 SortLayout sort_layout(uint32_t n);
 
-// Stable LSD radix sort of n (key, value) pairs by the low `bits` bits of the
-// 32-bit key (the others zero): 8-bit passes over one unit.  keys[cur] / vals[cur] hold the input; on return
+// Stable LSD radix sort of n (key, value) pairs by the whole 32-bit key: four
+// 8-bit passes over one unit.  keys[cur] / vals[cur] hold the input; on return
 // cur names the pair of buffers holding the result.  hist holds
 // radix_hist_entries(n) words, totals 256.
 size_t radix_hist_entries(uint32_t n);
 cudaError_t launch_radix_sort_pairs(uint32_t *const keys[2], uint32_t *const vals[2], uint32_t n, uint32_t *hist,
-                                    uint32_t *totals, int &cur, cudaStream_t stream, int bits = 32);
+                                    uint32_t *totals, int &cur, cudaStream_t stream);
 
 // Table rows at given ids and the table's gradient (rows.cu).  dtype, itype:
 // SDFOAM_F32 / F16 / BF16, SDFOAM_I32 (also unsigned) / I64; ld in elements.

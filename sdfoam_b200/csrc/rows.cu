@@ -16,9 +16,9 @@
 //     a row of the result whenever the id changes;
 //   * a segment that crosses a chunk's end leaves its parts in the workspace
 //     (at most two per chunk), and a second launch adds them in order;
-//   * rows that no id names are written as zeros by blocks of the same
-//     launch, from a byte per row that the sort's first pass sets -- the
-//     result is written exactly once.
+//   * rows that no id names are written as zeros by more blocks of that
+//     launch, from a byte per row that the sums set -- the result is written
+//     exactly once.
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -124,21 +124,280 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 }
 
 // --------------------------------------------------------------------------
-// gradient: keys
+// gradient: a stable sort of (row, position)
 // --------------------------------------------------------------------------
+//
+// Least significant digit first, digits of at most 9 bits (as few passes as
+// the number of rows needs, of equal width).  A pass over tiles of 4096
+// counts the digits of each tile, scans the counts, and scatters: every warp
+// ranks its 512 consecutive entries with __match_any_sync and its own digit
+// counts, the tile is put in order in shared memory and leaves in runs of
+// equal digits.  The first pass reads the ids themselves.  Up to 8192 entries
+// are sorted by one block in one launch.
 
-// keys[i] = the row id i names, or `rows` (sorts last); vals[i] = i; touched
-// rows are marked.
+constexpr int kSortThreads = 256;
+constexpr int kSortItems = 16;
+constexpr uint32_t kSortTile = kSortThreads * kSortItems;
+constexpr int kMaxBins = 512;
+constexpr uint32_t kBlockSort = 8192;  // entries that one block sorts
+
+uint32_t sort_tiles(uint32_t n) { return (n + kSortTile - 1) / kSortTile; }
+
+struct SortPass {
+    const void *ids;               // the first pass's input
+    const uint32_t *keys_in, *vals_in;
+    uint32_t *keys_out, *vals_out;
+    uint32_t *counts;              // [bins][tiles], then its exclusive scan along the tiles
+    uint32_t *totals;              // [bins]
+    uint32_t n, rows, tiles;
+    int shift, bins;
+    unsigned char *touched;        // cleared by the first pass
+};
+
+template <typename I, bool FIRST>
+__device__ __forceinline__ uint32_t sort_key(const SortPass &P, uint32_t i) {
+    if constexpr (FIRST) return row_of(static_cast<const I *>(P.ids)[i], P.rows);
+    else return P.keys_in[i];
+}
+
+// Clears bytes [block * share, ...) of the rows' marks.
+__device__ __forceinline__ void clear_touched(unsigned char *touched, uint32_t rows, uint32_t block, uint32_t blocks) {
+    const uint64_t words = (uint64_t(rows) + 15) / 16;  // the array is padded to 256 bytes
+    for (uint64_t w = uint64_t(block) * blockDim.x + threadIdx.x; w < words; w += uint64_t(blocks) * blockDim.x)
+        reinterpret_cast<uint4 *>(touched)[w] = make_uint4(0, 0, 0, 0);
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const SortPass P) {
+    __shared__ uint32_t count[kMaxBins];
+    for (int b = threadIdx.x; b < P.bins; b += kSortThreads) count[b] = 0;
+    if (FIRST) clear_touched(P.touched, P.rows, blockIdx.x, gridDim.x);
+    __syncthreads();
+    const uint32_t base = blockIdx.x * kSortTile, mask = P.bins - 1;
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r) {
+        const uint32_t i = base + r * kSortThreads + threadIdx.x;
+        // many entries of a warp may share a digit: one addition each
+        const uint32_t d = i < P.n ? (sort_key<I, FIRST>(P, i) >> P.shift) & mask : 0xffffffffu;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        if (i < P.n && (peers & ((1u << (threadIdx.x & 31)) - 1u)) == 0) atomicAdd(&count[d], __popc(peers));
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < P.bins; b += kSortThreads) P.counts[size_t(b) * P.tiles + blockIdx.x] = count[b];
+}
+
+// Exclusive scan of each digit's counts along the tiles, one warp per digit.
+__global__ void __launch_bounds__(256) scan_counts_kernel(const SortPass P) {
+    const uint32_t b = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (b >= uint32_t(P.bins)) return;
+    uint32_t *row = P.counts + size_t(b) * P.tiles;
+    uint32_t carry = 0;
+    for (uint32_t t0 = 0; t0 < P.tiles; t0 += 128) {
+        uint32_t v[4], incl[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t t = t0 + q * 32 + lane;
+            v[q] = t < P.tiles ? row[t] : 0u;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            incl[q] = v[q];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, incl[q], o);
+                if (lane >= uint32_t(o)) incl[q] += y;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t t = t0 + q * 32 + lane;
+            if (t < P.tiles) row[t] = carry + incl[q] - v[q];
+            carry += __shfl_sync(0xffffffffu, incl[q], 31);
+        }
+    }
+    if (lane == 0) P.totals[b] = carry;
+}
+
+// Ranks WARPS x ITEMS x 32 entries (warp w's are consecutive) by their digit
+// and puts them in order in shared memory: rank[] are this thread's places.
+// counts: [WARPS][bins], start: [bins + 1] first place of each digit.
+template <int WARPS, int ITEMS>
+__device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint32_t (&rank)[ITEMS], uint16_t *counts,
+                                            uint32_t *start, uint32_t *warp_sums, int bins) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lt = (1u << lane) - 1u;
+    constexpr uint32_t kThreads = WARPS * 32;
+    for (uint32_t i = threadIdx.x; i < uint32_t(WARPS * bins); i += kThreads) counts[i] = 0;
+    __syncthreads();
+    uint16_t *mine = counts + warp * bins;
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r) {
+        const uint32_t d = digit[r];
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        uint32_t before = 0;
+        if (d < uint32_t(bins)) before = mine[d];
+        __syncwarp();
+        if (d < uint32_t(bins) && (peers & lt) == 0) mine[d] = uint16_t(before + __popc(peers));
+        __syncwarp();
+        rank[r] = before + __popc(peers & lt);
+    }
+    __syncthreads();
+    // per digit: where each warp's entries start within the digit, and the
+    // digit's total; then the digits' starts
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < bins; b0 += int(kThreads)) {
+        const int b = b0 + int(threadIdx.x);
+        uint32_t total = 0;
+        if (b < bins) {
+#pragma unroll 8
+            for (int w = 0; w < WARPS; ++w) {
+                const uint32_t c = counts[w * bins + b];
+                counts[w * bins + b] = uint16_t(total);
+                total += c;
+            }
+        }
+        uint32_t incl = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= uint32_t(o)) incl += y;
+        }
+        if (lane == 31) warp_sums[warp] = incl;
+        __syncthreads();
+        uint32_t before = carry, all = 0;
+#pragma unroll 8
+        for (int w = 0; w < WARPS; ++w) {
+            if (uint32_t(w) < warp) before += warp_sums[w];
+            all += warp_sums[w];
+        }
+        if (b < bins) start[b] = before + incl - total;
+        carry += all;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < ITEMS; ++r)
+        if (digit[r] < uint32_t(bins)) rank[r] += mine[digit[r]] + start[digit[r]];
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const SortPass P) {
+    constexpr int kWarps = kSortThreads / 32;
+    __shared__ uint32_t keys[kSortTile];
+    __shared__ union {
+        uint16_t counts[kWarps * kMaxBins];
+        uint32_t vals[kSortTile / 2];  // half of the tile's at a time
+    } u;
+    __shared__ uint32_t start[kMaxBins], base[kMaxBins], warp_sums[kWarps];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mask = P.bins - 1;
+    const uint32_t tile0 = blockIdx.x * kSortTile, valid = min(kSortTile, P.n - tile0);
+    const uint32_t first = warp * (32 * kSortItems) + lane;
+    uint32_t key[kSortItems], digit[kSortItems], rank[kSortItems];
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r) {
+        const uint32_t i = first + r * 32;
+        key[r] = i < valid ? sort_key<I, FIRST>(P, tile0 + i) : 0u;
+        digit[r] = i < valid ? (key[r] >> P.shift) & mask : 0xffffffffu;
+    }
+    rank_digits<kWarps, kSortItems>(digit, rank, u.counts, start, warp_sums, P.bins);
+    // the digit's first place in the output: entries of smaller digits, this
+    // digit's in earlier tiles, less the tile's own start
+    __syncthreads();
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < P.bins; b0 += kSortThreads) {
+        const int b = b0 + int(threadIdx.x);
+        const uint32_t total = b < P.bins ? P.totals[b] : 0u;
+        uint32_t incl = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= uint32_t(o)) incl += y;
+        }
+        if (lane == 31) warp_sums[warp] = incl;
+        __syncthreads();
+        uint32_t before = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (uint32_t(w) < warp) before += warp_sums[w];
+            all += warp_sums[w];
+        }
+        if (b < P.bins) base[b] = before + incl - total + P.counts[size_t(b) * P.tiles + blockIdx.x] - start[b];
+        carry += all;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < kSortItems; ++r)
+        if (first + r * 32 < valid) keys[rank[r]] = key[r];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < valid; i += kSortThreads) {
+        const uint32_t k = keys[i], at = base[(k >> P.shift) & mask] + i;
+        if (at < P.n) P.keys_out[at] = k;  // always, for consistent counts; keeps the store in bounds
+    }
+    // the values, half of the places at a time, by the order of their keys
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSortItems; ++r) {
+            const uint32_t i = first + r * 32;
+            if (i < valid && rank[r] / (kSortTile / 2) == h)
+                u.vals[rank[r] % (kSortTile / 2)] = FIRST ? tile0 + i : P.vals_in[tile0 + i];
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kSortTile / 2 && h * (kSortTile / 2) + i < valid; i += kSortThreads) {
+            const uint32_t place = h * (kSortTile / 2) + i, at = base[(keys[place] >> P.shift) & mask] + place;
+            if (at < P.n) P.vals_out[at] = u.vals[i];
+        }
+    }
+}
+
+// Up to kBlockSort entries: block 0 sorts them, digits of 8 bits; the others
+// clear the rows' marks.
+constexpr int kBlockSortThreads = 1024;
+constexpr int kBlockSortBins = 256;
+constexpr size_t kBlockSortSmem = kBlockSort * 8 + kBlockSortThreads / 32 * kBlockSortBins * 2 + kBlockSortBins * 4 + 128;
+
 template <typename I>
-__global__ void __launch_bounds__(256) row_keys_kernel(const I *__restrict__ ids, uint32_t n, uint32_t rows,
-                                                       uint32_t *__restrict__ keys, uint32_t *__restrict__ vals,
-                                                       unsigned char *__restrict__ touched) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t k = row_of(ids[i], rows);
-    keys[i] = k;
-    vals[i] = i;
-    if (k < rows) touched[k] = 1;
+__global__ void __launch_bounds__(kBlockSortThreads) sort_block_kernel(const SortPass P, int bits) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    if (blockIdx.x > 0) {
+        clear_touched(P.touched, P.rows, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    constexpr int kWarps = kBlockSortThreads / 32, kItems = kBlockSort / kBlockSortThreads;
+    uint32_t *keys = reinterpret_cast<uint32_t *>(raw), *vals = keys + kBlockSort;
+    uint16_t *counts = reinterpret_cast<uint16_t *>(vals + kBlockSort);
+    uint32_t *start = reinterpret_cast<uint32_t *>(counts + kWarps * kBlockSortBins), *warp_sums = start + kBlockSortBins;
+    const uint32_t first = (threadIdx.x >> 5) * (32 * kItems) + (threadIdx.x & 31);
+    uint32_t key[kItems], val[kItems], digit[kItems], rank[kItems];
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+        val[r] = first + r * 32;
+        key[r] = val[r] < P.n ? sort_key<I, true>(P, val[r]) : 0u;
+    }
+    for (int shift = 0; shift < bits; shift += 8) {
+#pragma unroll
+        for (int r = 0; r < kItems; ++r)
+            digit[r] = first + r * 32 < P.n ? (key[r] >> shift) & (kBlockSortBins - 1) : 0xffffffffu;
+        rank_digits<kWarps, kItems>(digit, rank, counts, start, warp_sums, kBlockSortBins);
+#pragma unroll
+        for (int r = 0; r < kItems; ++r)
+            if (first + r * 32 < P.n) {
+                keys[rank[r]] = key[r];
+                vals[rank[r]] = val[r];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kItems; ++r)
+            if (first + r * 32 < P.n) {
+                key[r] = keys[first + r * 32];
+                val[r] = vals[first + r * 32];
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < kItems; ++r)
+        if (first + r * 32 < P.n) {
+            P.keys_out[first + r * 32] = key[r];
+            P.vals_out[first + r * 32] = val[r];
+        }
 }
 
 // --------------------------------------------------------------------------
@@ -147,7 +406,6 @@ __global__ void __launch_bounds__(256) row_keys_kernel(const I *__restrict__ ids
 
 constexpr int kSumThreads = 256;
 constexpr int kAhead = 4;            // rows in flight per lane and unit
-constexpr uint32_t kNoPart = 0xffffffffu;
 
 struct SumParams {
     const uint32_t *keys, *vals;  // sorted
@@ -160,13 +418,13 @@ struct SumParams {
     uint32_t chunk, chunks;       // entries per chunk, number of chunks
     float scale;
     char *out;                    // [rows][units] contiguous
-    const unsigned char *touched;
+    unsigned char *touched;       // [rows]: 1 for the rows that an id names
     float *parts;                 // [2 * chunks][columns]: the chunk's first and last segment
     uint32_t columns;             // elements per row
-    uint32_t sum_blocks;          // blocks of sums; the others write zero rows
+    uint32_t join_blocks;         // of the join's launch; the others write zero rows
 };
 
-// The blocks behind the sums': zeros for the rows that no id names.
+// The blocks behind the join's: zeros for the rows that no id names.
 template <int VB>
 __device__ __forceinline__ void zero_rows(const SumParams &P, uint32_t block, uint32_t blocks) {
     using W = typename Word<VB>::type;
@@ -193,10 +451,6 @@ template <typename T, int VB, int R>
 __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P) {
     using W = typename Word<VB>::type;
     constexpr int E = VB / int(sizeof(T));
-    if (blockIdx.x >= P.sum_blocks) {
-        if (blockIdx.y == 0) zero_rows<VB>(P, blockIdx.x - P.sum_blocks, gridDim.x - P.sum_blocks);
-        return;
-    }
     const uint32_t lanes = 1u << P.lane_bits, lane = threadIdx.x & (lanes - 1);
     const uint32_t c = blockIdx.x * (kSumThreads >> P.lane_bits) + (threadIdx.x >> P.lane_bits);
     if (c >= P.chunks) return;
@@ -214,6 +468,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P
 
     auto flush = [&](uint32_t key, bool more) {
         if (key >= P.rows) return;  // ids that name no row
+        if (lane == 0 && blockIdx.y == 0) P.touched[key] = 1;
         if (open || more) {
             float *part = P.parts + size_t(2 * c + (open ? 0 : 1)) * P.columns;
 #pragma unroll
@@ -276,54 +531,81 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P
 
 // Adds the parts of the segments that cross chunk ends.  The chunk a segment
 // starts in owns it: its last part, then the first parts of the chunks that
-// follow while they continue the segment.  A block takes kJoinChunks chunks;
-// segments of many chunks (hot ids) are shared by the block's threads, each
-// taking a contiguous run of the parts, and their sums are added in order.
+// follow while they continue the segment.  A warp looks at one chunk and adds
+// a segment of few chunks itself; segments of many (hot ids) are shared by
+// the block's threads, each taking a contiguous run of the parts, and the
+// runs' sums are added in order.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinChunks = 8;
-constexpr int kJoinSlices = 16;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr uint32_t kJoinSlices = 16;
+constexpr uint32_t kJoinLong = 64;  // chunks that a warp adds alone
 
-template <typename T>
+template <typename T, int VB>
 __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const SumParams P) {
-    __shared__ float partial[kJoinSlices][kJoinThreads / kJoinSlices];
+    if (blockIdx.x >= P.join_blocks) {
+        zero_rows<VB>(P, blockIdx.x - P.join_blocks, gridDim.x - P.join_blocks);
+        return;
+    }
     constexpr uint32_t kCols = kJoinThreads / kJoinSlices;  // columns of a slice's threads
-    const uint32_t slice = threadIdx.x / kCols, tc = threadIdx.x % kCols;
-    for (uint32_t i = 0; i < uint32_t(kJoinChunks); ++i) {
-        const uint32_t c = blockIdx.x * kJoinChunks + i;
-        if (c + 1 >= P.chunks) return;
+    __shared__ float partial[kJoinSlices][kCols];
+    __shared__ uint32_t long_key[kJoinWarps], long_count[kJoinWarps];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t c = blockIdx.x * kJoinWarps + warp;
+    if (lane == 0) long_count[warp] = 0;
+    if (c + 1 < P.chunks) {
         const uint32_t end = (c + 1) * P.chunk, beg = end - P.chunk;
         const uint32_t key = P.keys[end - 1];
-        if (key >= P.rows || P.keys[end] != key) continue;                             // nothing crosses this end
-        if (beg > 0 && P.keys[beg] == key && P.keys[beg - 1] == key) continue;         // another chunk owns it
-        // last chunk with entries of this segment: the first entry past it by bisection
-        uint32_t lo = end, hi = P.n;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (P.keys[mid] <= key) lo = mid + 1;
-            else hi = mid;
-        }
-        const uint32_t last = (lo - 1) / P.chunk;
-        const uint32_t count = last - c;  // first parts of chunks c + 1 .. last
-        if (count < 4 * kJoinSlices) {
-            for (uint32_t col = threadIdx.x; col < P.columns; col += kJoinThreads) {
-                float s = P.parts[size_t(2 * c + 1) * P.columns + col];
-                for (uint32_t k = 1; k <= count; ++k) s += P.parts[size_t(2 * (c + k)) * P.columns + col];
-                reinterpret_cast<T *>(P.out)[size_t(key) * P.columns + col] = from_f<T>(P.scale * s);
+        // a segment of a row crosses this end, and starts in this chunk
+        if (key < P.rows && P.keys[end] == key && (beg == 0 || P.keys[beg] != key || P.keys[beg - 1] != key)) {
+            // first parts of chunks c + 1 .. c + count: the chunks that the
+            // segment fills, and the one it ends in
+            uint32_t count = 1;
+            const uint64_t far = uint64_t(end) + uint64_t(lane + 1) * P.chunk;  // end of chunk c + 1 + lane
+            const bool on = far < P.n && P.keys[far] == key;
+            const uint32_t filled = __ballot_sync(0xffffffffu, !on);
+            if (filled) {
+                count += __ffs(filled) - 1;
+            } else {
+                uint32_t lo = end, hi = P.n;  // the first entry past the segment, by bisection
+                while (lo < hi) {
+                    const uint32_t mid = lo + (hi - lo) / 2;
+                    if (P.keys[mid] <= key) lo = mid + 1;
+                    else hi = mid;
+                }
+                count = (lo - 1) / P.chunk - c;
             }
-            continue;
+            if (count <= kJoinLong) {
+                for (uint32_t col = lane; col < P.columns; col += 32) {
+                    float s = P.parts[size_t(2 * c + 1) * P.columns + col];
+#pragma unroll 4
+                    for (uint32_t k = 1; k <= count; ++k) s += P.parts[size_t(2) * (c + k) * P.columns + col];
+                    reinterpret_cast<T *>(P.out)[size_t(key) * P.columns + col] = from_f<T>(P.scale * s);
+                }
+            } else if (lane == 0) {
+                long_key[warp] = key;
+                long_count[warp] = count;
+            }
         }
+    }
+    __syncthreads();
+    const uint32_t slice = threadIdx.x / kCols, tc = threadIdx.x % kCols;
+    for (uint32_t w = 0; w < uint32_t(kJoinWarps); ++w) {
+        const uint32_t count = long_count[w], key = long_key[w], from = blockIdx.x * kJoinWarps + w;
+        if (count == 0) continue;  // the same for every thread
         const uint32_t per = (count + kJoinSlices - 1) / kJoinSlices;
         const uint32_t k0 = 1 + slice * per, k1 = min(count + 1, k0 + per);
         for (uint32_t col0 = 0; col0 < P.columns; col0 += kCols) {
             const uint32_t col = col0 + tc;
             float s = 0.0f;
-            if (col < P.columns)
-                for (uint32_t k = k0; k < k1; ++k) s += P.parts[size_t(2 * (c + k)) * P.columns + col];
+            if (col < P.columns) {
+#pragma unroll 8
+                for (uint32_t k = k0; k < k1; ++k) s += P.parts[size_t(2) * (from + k) * P.columns + col];
+            }
             partial[slice][tc] = s;
             __syncthreads();
             if (slice == 0 && col < P.columns) {
-                float t = P.parts[size_t(2 * c + 1) * P.columns + col];
-                for (int q = 0; q < kJoinSlices; ++q) t += partial[q][tc];
+                float t = P.parts[size_t(2 * from + 1) * P.columns + col];
+                for (uint32_t q = 0; q < kJoinSlices; ++q) t += partial[q][tc];
                 reinterpret_cast<T *>(P.out)[size_t(key) * P.columns + col] = from_f<T>(P.scale * t);
             }
             __syncthreads();
@@ -353,7 +635,7 @@ uint32_t chunk_of(uint32_t n) {
 }
 
 struct RowGradLayout {
-    size_t keys[2], vals[2], hist, totals, touched, parts, total;
+    size_t keys[2], vals[2], counts, totals, touched, parts, total;
     uint32_t chunk, chunks;
 };
 
@@ -369,8 +651,8 @@ RowGradLayout grad_layout(uint32_t n, uint32_t rows, uint32_t columns) {
         l.keys[i] = take(size_t(n) * 4);
         l.vals[i] = take(size_t(n) * 4);
     }
-    l.hist = take(radix_hist_entries(n) * 4);
-    l.totals = take(256 * 4);
+    l.counts = take(size_t(kMaxBins) * sort_tiles(n) * 4);
+    l.totals = take(kMaxBins * 4);
     l.touched = take(rows);
     l.chunk = chunk_of(n);
     l.chunks = (n + l.chunk - 1) / l.chunk;
@@ -429,15 +711,49 @@ cudaError_t sum_typed(SumParams &P, cudaStream_t stream) {
     const int R = per_lane >= 3 && VB < 16 ? 4 : per_lane >= 2 ? 2 : 1;
     P.lane_units = int(lanes) * R;
     const uint32_t groups = kSumThreads / lanes;
-    P.sum_blocks = (P.chunks + groups - 1) / groups;
-    const uint64_t zero_units = uint64_t(P.rows) * P.units;
-    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 2047) / 2048, 148 * 4));
-    const dim3 grid(P.sum_blocks + zero_blocks, (P.units + P.lane_units - 1) / P.lane_units);
+    const dim3 grid((P.chunks + groups - 1) / groups, (P.units + P.lane_units - 1) / P.lane_units);
     if (R == 4) sum_rows_kernel<T, VB, (VB < 16 ? 4 : 2)><<<grid, kSumThreads, 0, stream>>>(P);
     else if (R == 2) sum_rows_kernel<T, VB, 2><<<grid, kSumThreads, 0, stream>>>(P);
     else sum_rows_kernel<T, VB, 1><<<grid, kSumThreads, 0, stream>>>(P);
-    if (P.chunks > 1)
-        join_parts_kernel<T><<<(P.chunks + kJoinChunks - 1) / kJoinChunks, kJoinThreads, 0, stream>>>(P);
+    P.join_blocks = (P.chunks + kJoinWarps - 1) / kJoinWarps;
+    const uint64_t zero_units = uint64_t(P.rows) * P.units;
+    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 2047) / 2048, 148 * 8));
+    join_parts_kernel<T, VB><<<P.join_blocks + zero_blocks, kJoinThreads, 0, stream>>>(P);
+    return cudaGetLastError();
+}
+
+template <typename I>
+cudaError_t sort_ids(SortPass &P, uint32_t *const keys[2], uint32_t *const vals[2], int &cur, cudaStream_t stream) {
+    int bits = 0;  // of the largest key, `rows`
+    while (bits < 32 && (uint64_t(P.rows) >> bits) != 0) ++bits;
+    if (P.n <= kBlockSort) {
+        cudaError_t e = cudaFuncSetAttribute(sort_block_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             int(kBlockSortSmem));
+        if (e != cudaSuccess) return e;
+        cur = 0;
+        P.keys_out = keys[0];
+        P.vals_out = vals[0];
+        const unsigned clear = unsigned(std::min<uint64_t>((uint64_t(P.rows) + 16383) / 16384, 147));
+        sort_block_kernel<I><<<1 + clear, kBlockSortThreads, kBlockSortSmem, stream>>>(P, bits);
+        return cudaGetLastError();
+    }
+    const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes;
+    P.tiles = sort_tiles(P.n);
+    P.bins = 1 << width;
+    cur = 0;
+    for (int p = 0; p < passes; ++p) {
+        P.shift = p * width;
+        P.keys_in = keys[cur ^ 1];
+        P.vals_in = vals[cur ^ 1];
+        P.keys_out = keys[cur];
+        P.vals_out = vals[cur];
+        if (p == 0) digit_counts_kernel<I, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        else digit_counts_kernel<I, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        scan_counts_kernel<<<(P.bins + 7) / 8, 256, 0, stream>>>(P);
+        if (p == 0) scatter_digits_kernel<I, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        else scatter_digits_kernel<I, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        if (p + 1 < passes) cur ^= 1;
+    }
     return cudaGetLastError();
 }
 
@@ -486,18 +802,16 @@ cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t co
         vals[i] = reinterpret_cast<uint32_t *>(ws + l.vals[i]);
     }
     unsigned char *touched = reinterpret_cast<unsigned char *>(ws + l.touched);
-    cudaError_t e = cudaMemsetAsync(touched, 0, rows, stream);
-    if (e != cudaSuccess) return e;
-    const unsigned blocks = (n + 255) / 256;
-    if (itype == SDFOAM_I64)
-        row_keys_kernel<<<blocks, 256, 0, stream>>>(static_cast<const long long *>(ids), n, rows, keys[0], vals[0], touched);
-    else
-        row_keys_kernel<<<blocks, 256, 0, stream>>>(static_cast<const uint32_t *>(ids), n, rows, keys[0], vals[0], touched);
-    int bits = 0;  // of the largest key, `rows`
-    while (bits < 32 && (uint64_t(rows) >> bits) != 0) ++bits;
+    SortPass S{};
+    S.ids = ids;
+    S.counts = reinterpret_cast<uint32_t *>(ws + l.counts);
+    S.totals = reinterpret_cast<uint32_t *>(ws + l.totals);
+    S.n = n;
+    S.rows = rows;
+    S.touched = touched;
     int cur = 0;
-    e = launch_radix_sort_pairs(keys, vals, n, reinterpret_cast<uint32_t *>(ws + l.hist),
-                                reinterpret_cast<uint32_t *>(ws + l.totals), cur, stream, bits);
+    const cudaError_t e = itype == SDFOAM_I64 ? sort_ids<long long>(S, keys, vals, cur, stream)
+                                              : sort_ids<uint32_t>(S, keys, vals, cur, stream);
     if (e != cudaSuccess) return e;
     SumParams P{};
     P.keys = keys[cur];

@@ -103,7 +103,9 @@ def test_lookup_shapes_and_strides():
 @pytest.mark.parametrize("columns", [1, 2, 3, 49, 256, 700])
 def test_gradient(dtype, columns):
     g = torch.Generator(device="cuda").manual_seed(columns)
-    for n, rows in ((1, 1), (5, 300), (127, 5), (1000, 70000), (4097, 256), (20000, 255), (30011, 66000)):
+    # one block sorts up to 8192 ids; more take passes of up to 9 bits
+    for n, rows in ((1, 1), (5, 300), (127, 5), (1000, 70000), (4097, 256), (8192, 65536), (8193, 1), (20000, 255),
+                    (20000, 512), (30011, 66000), (9000, 300000)):
         v = torch.randint(-2, rows + 2, (n,), generator=g, device="cuda")
         grad = torch.randn((n, columns), generator=g, device="cuda").to(dtype)
         for index in (torch.uint32, torch.int64):
@@ -124,8 +126,8 @@ def test_gradient_of_hot_rows(columns):
     for v, rows in ((torch.zeros_like(at), 1), (torch.full_like(at, 9), 1000), (at % 3 * 40, 100), (at // 32, n),
                     (at // 1024 + 5, n), (torch.full_like(at, -1), 50), (torch.where(at < n - 1, 3, 4), 6)):
         got = foam.lookup_rows_backward(grad, v, rows)
-        # sums of chunks of at most 128, of slices of parts, of slices
-        check_gradient(got, grad, v, rows, 1.0, 128 + n // 128 // 16 + 32)
+        # chunks of 4 to 128 rows, then their sums in 16 runs, then the runs
+        check_gradient(got, grad, v, rows, 1.0, 128 + n // 4 // 16 + 1 + 17)
         assert torch.equal(got, foam.lookup_rows_backward(grad, v, rows)), "not the same bits"
 
 
