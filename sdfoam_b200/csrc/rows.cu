@@ -84,26 +84,46 @@ union Unit {
 
 constexpr int kLookupThreads = 256;
 
-// Units of VB bytes in the flat order of the output, ITEMS per thread: the
-// block's first unit is divided by the units per row in 64 bits, the rest of
-// the positions follow from 32-bit offsets.  Consecutive lanes write
-// consecutive units whatever the row length.
+// x / d and x % d, in 32 bits where x allows.
+__device__ __forceinline__ uint64_t divide(uint64_t x, uint32_t d, uint32_t &rem) {
+    if (x >> 32) {
+        const uint64_t q = x / d;
+        rem = uint32_t(x - q * d);
+        return q;
+    }
+    const uint32_t q = uint32_t(x) / d;
+    rem = uint32_t(x) - q * d;
+    return q;
+}
+
+// Units of VB bytes in the flat order of the output, ITEMS per thread, 256
+// apart: consecutive lanes write consecutive units whatever the row length.
+// A thread divides its first unit by the units per row; the others follow by
+// step_row rows and step_col units (256 divided by the units per row).
 template <typename T, typename I, int VB, int ITEMS>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__restrict__ table, uint32_t rows,
                                                                 size_t row_bytes, const I *__restrict__ ids,
-                                                                uint64_t total, uint32_t units, float scale,
+                                                                uint64_t total, uint32_t units, uint32_t step_row,
+                                                                uint32_t step_col, float scale,
                                                                 char *__restrict__ out) {
     using W = typename Word<VB>::type;
     const uint64_t first = uint64_t(blockIdx.x) * (kLookupThreads * ITEMS);
-    const uint64_t row0 = first / units;
-    const uint32_t col0 = uint32_t(first - row0 * units);
     uint32_t col[ITEMS], row[ITEMS];
+    {
+        uint32_t c;
+        const uint64_t r0 = divide(first + threadIdx.x, units, c);
+        const I *id = ids + r0;
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-        const uint32_t e = col0 + j * kLookupThreads + threadIdx.x;  // < units + 2048: fits
-        const uint32_t r = e / units;
-        col[j] = e - r * units;
-        row[j] = first + j * kLookupThreads + threadIdx.x < total ? row_of(ids[row0 + r], rows) : rows;
+        for (int j = 0; j < ITEMS; ++j) {
+            col[j] = c;
+            row[j] = first + j * kLookupThreads + threadIdx.x < total ? row_of(*id, rows) : rows;
+            c += step_col;
+            id += step_row;
+            if (c >= units) {
+                c -= units;
+                ++id;
+            }
+        }
     }
     Unit<T, VB> u[ITEMS];
 #pragma unroll
@@ -119,7 +139,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
             for (int e = 0; e < int(VB / sizeof(T)); ++e)
                 if (row[j] < rows) u[j].item[e] = from_f<T>(scale * to_f<T>(u[j].item[e]));
         }
-        if (first + j * kLookupThreads + threadIdx.x < total) dst[j * kLookupThreads] = u[j].word;
+        if (first + j * kLookupThreads + threadIdx.x < total) __stcs(dst + j * kLookupThreads, u[j].word);
     }
 }
 
@@ -128,15 +148,15 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 // --------------------------------------------------------------------------
 //
 // Least significant digit first, digits of at most 9 bits (as few passes as
-// the number of rows needs, of equal width).  A pass over tiles of 4096
+// the number of rows needs, of equal width).  A pass over tiles of 2048
 // counts the digits of each tile, scans the counts, and scatters: every warp
-// ranks its 512 consecutive entries with __match_any_sync and its own digit
-// counts, the tile is put in order in shared memory and leaves in runs of
+// ranks its 256 consecutive entries by ballots over the digit's bits and its
+// own digit counts (__match_any_sync took 360 cycles a call here), the tile is put in order in shared memory and leaves in runs of
 // equal digits.  The first pass reads the ids themselves.  Up to 8192 entries
 // are sorted by one block in one launch.
 
 constexpr int kSortThreads = 256;
-constexpr int kSortItems = 16;
+constexpr int kSortItems = 8;
 constexpr uint32_t kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxBins = 512;
 constexpr uint32_t kBlockSort = 8192;  // entries that one block sorts
@@ -177,10 +197,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const SortPa
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
         const uint32_t i = base + r * kSortThreads + threadIdx.x;
-        // many entries of a warp may share a digit: one addition each
-        const uint32_t d = i < P.n ? (sort_key<I, FIRST>(P, i) >> P.shift) & mask : 0xffffffffu;
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);
-        if (i < P.n && (peers & ((1u << (threadIdx.x & 31)) - 1u)) == 0) atomicAdd(&count[d], __popc(peers));
+        if (i < P.n) atomicAdd(&count[(sort_key<I, FIRST>(P, i) >> P.shift) & mask], 1u);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < P.bins; b += kSortThreads) P.counts[size_t(b) * P.tiles + blockIdx.x] = count[b];
@@ -218,12 +235,25 @@ __global__ void __launch_bounds__(256) scan_counts_kernel(const SortPass P) {
     if (lane == 0) P.totals[b] = carry;
 }
 
+// The lanes whose digit (of at most 9 bits) is this lane's, among the valid ones.
+__device__ __forceinline__ uint32_t same_digit(uint32_t digit, bool valid, int width) {
+    uint32_t peers = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+    for (int b = 0; b < 9; ++b) {
+        if (b >= width) break;
+        const uint32_t set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
+        peers &= (digit >> b) & 1u ? set : ~set;
+    }
+    return peers;
+}
+
 // Ranks WARPS x ITEMS x 32 entries (warp w's are consecutive) by their digit
 // and puts them in order in shared memory: rank[] are this thread's places.
 // counts: [WARPS][bins], start: [bins + 1] first place of each digit.
 template <int WARPS, int ITEMS>
 __device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint32_t (&rank)[ITEMS], uint16_t *counts,
                                             uint32_t *start, uint32_t *warp_sums, int bins) {
+    const int width = 31 - __clz(bins);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lt = (1u << lane) - 1u;
     constexpr uint32_t kThreads = WARPS * 32;
     for (uint32_t i = threadIdx.x; i < uint32_t(WARPS * bins); i += kThreads) counts[i] = 0;
@@ -232,11 +262,12 @@ __device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
         const uint32_t d = digit[r];
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        const bool valid = d < uint32_t(bins);
+        const uint32_t peers = same_digit(d, valid, width);
         uint32_t before = 0;
-        if (d < uint32_t(bins)) before = mine[d];
+        if (valid) before = mine[d];
         __syncwarp();
-        if (d < uint32_t(bins) && (peers & lt) == 0) mine[d] = uint16_t(before + __popc(peers));
+        if (valid && (peers & lt) == 0) mine[d] = uint16_t(before + __popc(peers));
         __syncwarp();
         rank[r] = before + __popc(peers & lt);
     }
@@ -284,7 +315,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
     __shared__ uint32_t keys[kSortTile];
     __shared__ union {
         uint16_t counts[kWarps * kMaxBins];
-        uint32_t vals[kSortTile / 2];  // half of the tile's at a time
+        uint32_t vals[kSortTile];
     } u;
     __shared__ uint32_t start[kMaxBins], base[kMaxBins], warp_sums[kWarps];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mask = P.bins - 1;
@@ -331,21 +362,16 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
         const uint32_t k = keys[i], at = base[(k >> P.shift) & mask] + i;
         if (at < P.n) P.keys_out[at] = k;  // always, for consistent counts; keeps the store in bounds
     }
-    // the values, half of the places at a time, by the order of their keys
+    // the values, in the order of their keys (the counts are no longer needed)
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kSortItems; ++r) {
-            const uint32_t i = first + r * 32;
-            if (i < valid && rank[r] / (kSortTile / 2) == h)
-                u.vals[rank[r] % (kSortTile / 2)] = FIRST ? tile0 + i : P.vals_in[tile0 + i];
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < kSortTile / 2 && h * (kSortTile / 2) + i < valid; i += kSortThreads) {
-            const uint32_t place = h * (kSortTile / 2) + i, at = base[(keys[place] >> P.shift) & mask] + place;
-            if (at < P.n) P.vals_out[at] = u.vals[i];
-        }
+    for (int r = 0; r < kSortItems; ++r) {
+        const uint32_t i = first + r * 32;
+        if (i < valid) u.vals[rank[r]] = FIRST ? tile0 + i : P.vals_in[tile0 + i];
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < valid; i += kSortThreads) {
+        const uint32_t at = base[(keys[i] >> P.shift) & mask] + i;
+        if (at < P.n) P.vals_out[at] = u.vals[i];
     }
 }
 
@@ -404,7 +430,11 @@ __global__ void __launch_bounds__(kBlockSortThreads) sort_block_kernel(const Sor
 // gradient: sums of sorted rows
 // --------------------------------------------------------------------------
 
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 128;
+constexpr int kJoinThreads = 512;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr uint32_t kJoinSlices = 32;
+constexpr uint32_t kJoinLong = 16;  // chunks that a warp adds alone
 constexpr int kAhead = 4;            // rows in flight per lane and unit
 
 struct SumParams {
@@ -430,15 +460,22 @@ __device__ __forceinline__ void zero_rows(const SumParams &P, uint32_t block, ui
     using W = typename Word<VB>::type;
     const uint64_t total = uint64_t(P.rows) * P.units;
     constexpr int kItems = 8;
-    const uint64_t step = uint64_t(blocks) * kSumThreads * kItems;
+    const uint64_t step = uint64_t(blocks) * kJoinThreads * kItems;
+    const uint32_t step_row = kJoinThreads / P.units, step_col = kJoinThreads % P.units;
     W *dst = reinterpret_cast<W *>(P.out);
-    for (uint64_t first = uint64_t(block) * kSumThreads * kItems; first < total; first += step) {
-        const uint64_t row0 = first / P.units;
-        const uint32_t col0 = uint32_t(first - row0 * P.units);
+    for (uint64_t first = uint64_t(block) * kJoinThreads * kItems; first < total; first += step) {
+        uint32_t col;
+        uint64_t row = divide(first + threadIdx.x, P.units, col);
 #pragma unroll
         for (int j = 0; j < kItems; ++j) {
-            const uint32_t e = j * kSumThreads + threadIdx.x;
-            if (first + e < total && !P.touched[row0 + (col0 + e) / P.units]) dst[first + e] = W{};
+            const uint64_t at = first + j * kJoinThreads + threadIdx.x;
+            if (at < total && !P.touched[row]) dst[at] = W{};
+            col += step_col;
+            row += step_row;
+            if (col >= P.units) {
+                col -= P.units;
+                ++row;
+            }
         }
     }
 }
@@ -492,21 +529,34 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P
         }
     };
 
+    // the entries of the next rows are read while these rows are on their way
+    uint32_t next_key[kAhead], next_val[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+        const uint32_t j = min(beg + a, end - 1);
+        next_key[a] = P.keys[j];
+        next_val[a] = P.vals[j];
+    }
     for (uint32_t j0 = beg; j0 < end; j0 += kAhead) {
         uint32_t key[kAhead];
         Unit<T, VB> w[kAhead][R];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-            const uint32_t j = min(j0 + a, end - 1);
-            key[a] = P.keys[j];
+            key[a] = next_key[a];
             const bool named = key[a] < P.rows && j0 + a < end;
-            const char *src = P.grad + size_t(P.vals[j]) * P.grad_bytes;
+            const char *src = P.grad + size_t(next_val[a]) * P.grad_bytes;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const uint32_t u = u0 + r * lanes;
                 w[a][r].word = W{};
-                if (named && u < P.units) w[a][r].word = *reinterpret_cast<const W *>(src + size_t(u) * VB);
+                if (named && u < P.units) w[a][r].word = __ldcs(reinterpret_cast<const W *>(src + size_t(u) * VB));
             }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const uint32_t j = min(j0 + kAhead + a, end - 1);
+            next_key[a] = P.keys[j];
+            next_val[a] = P.vals[j];
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
@@ -535,10 +585,6 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P
 // a segment of few chunks itself; segments of many (hot ids) are shared by
 // the block's threads, each taking a contiguous run of the parts, and the
 // runs' sums are added in order.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinWarps = kJoinThreads / 32;
-constexpr uint32_t kJoinSlices = 16;
-constexpr uint32_t kJoinLong = 64;  // chunks that a warp adds alone
 
 template <typename T, int VB>
 __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const SumParams P) {
@@ -566,13 +612,19 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const SumParam
             if (filled) {
                 count += __ffs(filled) - 1;
             } else {
-                uint32_t lo = end, hi = P.n;  // the first entry past the segment, by bisection
-                while (lo < hi) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    if (P.keys[mid] <= key) lo = mid + 1;
-                    else hi = mid;
+                // chunks c + 1 .. c + lo are filled; the first that is not by
+                // 32 places at a time
+                uint32_t lo = 32, hi = P.chunks - 1 - c;  // c + hi: at most the last chunk
+                while (hi - lo > 1) {
+                    const uint32_t step = (hi - lo + 31) / 32;
+                    const uint64_t k = uint64_t(lo) + uint64_t(lane + 1) * step;
+                    const uint64_t at = uint64_t(end) + k * P.chunk;
+                    const bool past = k >= hi || at >= P.n || P.keys[at] != key;
+                    const uint32_t f = __ffs(__ballot_sync(0xffffffffu, past));  // 1 + the first lane past
+                    hi = f ? min(uint64_t(hi), uint64_t(lo) + uint64_t(f) * step) : hi;
+                    lo = f ? lo + (f - 1) * step : lo + 32 * step;
                 }
-                count = (lo - 1) / P.chunk - c;
+                count = lo + 1;
             }
             if (count <= kJoinLong) {
                 for (uint32_t col = lane; col < P.columns; col += 32) {
@@ -627,10 +679,10 @@ int unit_bytes(const void *base, size_t stride, size_t bytes) {
 }
 
 // Entries per chunk: enough chunks to fill the GPU (a chunk is a warp or
-// less; 148 SMs x 64), and no more parts than needed.
+// less; 148 SMs x 128), and no more parts than needed.
 uint32_t chunk_of(uint32_t n) {
     uint32_t c = 4;
-    while (c < 128 && uint64_t(c) * 148 * 64 < n) c *= 2;
+    while (c < 64 && uint64_t(c) * 148 * 128 < n) c *= 2;
     return c;
 }
 
@@ -665,14 +717,18 @@ template <typename T, typename I, int VB>
 cudaError_t lookup_typed(const void *table, uint32_t rows, size_t row_bytes, const void *ids, uint64_t n,
                          uint32_t units, float scale, void *out, cudaStream_t stream) {
     const uint64_t total = n * units;
-    // few units: more blocks of fewer items
+    const uint32_t step_row = kLookupThreads / units, step_col = kLookupThreads % units;
+    // few units: more blocks of fewer items.  1M rows of 49 floats at skewed
+    // ids with 4, 8, 16 items: 102, 106, 111 us, and 97 us with 8 and streaming
+    // stores (the output does not push the table's hot rows out of L2); a
+    // warp per 8 rows, lanes along the row, takes 165.
     if (total < 148ull * 2048 * 4) {
         lookup_kernel<T, I, VB, 2><<<unsigned((total + 511) / 512), kLookupThreads, 0, stream>>>(
-            static_cast<const char *>(table), rows, row_bytes, static_cast<const I *>(ids), total, units, scale,
+            static_cast<const char *>(table), rows, row_bytes, static_cast<const I *>(ids), total, units, step_row, step_col, scale,
             static_cast<char *>(out));
     } else {
         lookup_kernel<T, I, VB, 8><<<unsigned((total + 2047) / 2048), kLookupThreads, 0, stream>>>(
-            static_cast<const char *>(table), rows, row_bytes, static_cast<const I *>(ids), total, units, scale,
+            static_cast<const char *>(table), rows, row_bytes, static_cast<const I *>(ids), total, units, step_row, step_col, scale,
             static_cast<char *>(out));
     }
     return cudaGetLastError();
@@ -717,7 +773,7 @@ cudaError_t sum_typed(SumParams &P, cudaStream_t stream) {
     else sum_rows_kernel<T, VB, 1><<<grid, kSumThreads, 0, stream>>>(P);
     P.join_blocks = (P.chunks + kJoinWarps - 1) / kJoinWarps;
     const uint64_t zero_units = uint64_t(P.rows) * P.units;
-    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 2047) / 2048, 148 * 8));
+    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 4095) / 4096, 148 * 4));
     join_parts_kernel<T, VB><<<P.join_blocks + zero_blocks, kJoinThreads, 0, stream>>>(P);
     return cudaGetLastError();
 }
