@@ -271,18 +271,27 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
     if (P.store == kStoreSpan) {
         // 16-bit rows of q_rows columns one after another, all groups
         asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
-        const uint32_t n = P.q_rows;
+        const uint32_t n = P.q_rows, left = n - min(n, col0), odd = (lane * n + col0) & 1u;
         uint16_t *dst = reinterpret_cast<uint16_t *>(row_stage) + lane * n + col0;
+        // whole words: a row that starts on half a word stores its first
+        // column alone and the pairs one column further
+        uint32_t w = 0, before = 0;
 #pragma unroll
-        for (int i = 0; i < kCols / 2; ++i) {
-            const float2 x = unpair(acc[i]);
-            const uint32_t w = pack2(P.out_dtype, x.x, x.y);
-            if (col0 + 2 * i + 1 < n && (n & 1u) == 0) {
-                *reinterpret_cast<uint32_t *>(dst + 2 * i) = w;
-            } else {
-                if (col0 + 2 * i < n) dst[2 * i] = uint16_t(w);
-                if (col0 + 2 * i + 1 < n) dst[2 * i + 1] = uint16_t(w >> 16);
+        for (int i = 0; i <= kCols / 2; ++i) {
+            if (i < kCols / 2) {
+                const float2 x = unpair(acc[i]);
+                w = pack2(P.out_dtype, x.x, x.y);
             }
+            // columns c and c + 1: 2 i and 2 i + 1, or 2 i - 1 and 2 i
+            const uint32_t pair = odd ? __byte_perm(before, w, 0x5432) : w;
+            const int c = 2 * i - int(odd);
+            if (i < kCols / 2 && c >= 0 && uint32_t(c) + 1 < left) {
+                *reinterpret_cast<uint32_t *>(dst + c) = pair;
+            } else {
+                if (c >= 0 && uint32_t(c) < left && c < kCols) dst[c] = uint16_t(pair);
+                if (i < kCols / 2 && c < 0 && left > 0) dst[0] = uint16_t(pair >> 16);
+            }
+            before = w;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
