@@ -66,192 +66,229 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Eight consecutive elements, zeros past k.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *src, int left, float *v) {
-    if (VEC && left >= 8) {
-        union Eight {
-            uint4 q[sizeof(T) / 2];
-            T e[8];
-            __device__ Eight() {}
-        } u;
+// Starts the copy of eight consecutive elements (zeros past `left`) into
+// this thread's place of the staging buffer.
+template <typename T>
+__device__ __forceinline__ void stage8(unsigned char *dst, const T *src, int left) {
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
 #pragma unroll
-        for (int i = 0; i < int(sizeof(T) / 2); ++i) u.q[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = as_float(u.e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? as_float(src[i]) : 0.0f;
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+        const int bytes = max(0, min(16, left * int(sizeof(T)) - 16 * i));
+        // a copy of nothing still needs an address of the matrix
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 16 * i),
+                     "l"(bytes > 0 ? reinterpret_cast<const char *>(src) + 16 * i : reinterpret_cast<const char *>(src)),
+                     "r"(bytes)
+                     : "memory");
     }
 }
 
-// One 128 x 128 tile per block.  Thread (g, c) holds rows 4 g .. 4 g + 3 and
-// columns 8 c .. 8 c + 7: a row of the tile is 16 lanes' 16-byte loads, and
-// the thread's 4 rows of one column are 4 consecutive bytes of the turned
+// 128 x 128 tiles, one after another.  Thread (g, c) holds rows 4 g .. 4 g + 3
+// and columns 8 c .. 8 c + 7: a row of the tile is 16 lanes' 16-byte copies,
+// and the thread's 4 rows of one column are 4 consecutive bytes of the turned
 // tile, which goes out through shared memory.  32 elements a thread keep it
-// at 64 registers, so that two blocks of 16 warps hide each other's loads.
+// at 64 registers, two blocks of 16 warps to an SM; the next tile's copies
+// (VEC: rows of 16-byte pieces) run while this one is worked on, each thread
+// reading only what it copied itself.
 template <typename T, bool VEC, int BLOCK_ROWS, bool NORMAL, bool TURNED>
 __global__ void __launch_bounds__(kThreads, 2) quantize_kernel(const QuantParams P) {
     constexpr int kWarps = kThreads / 32;
+    extern __shared__ __align__(16) unsigned char staged[];  // VEC: [2][kTile][kTile] of T
     __shared__ __align__(16) uint32_t tile[TURNED ? kTile * kTile / 4 : 4];
     __shared__ __align__(16) float tops[TURNED && BLOCK_ROWS == 1 ? kWarps : 1][kTile];
     __shared__ __align__(16) float inverses[TURNED && BLOCK_ROWS == 1 ? kTile : 4];
     __shared__ float top_all[kWarps];
     const uint32_t g = threadIdx.x >> 4, c = threadIdx.x & 15, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t kb = blockIdx.x % P.k_blocks, mb = blockIdx.x / P.k_blocks;
-    const uint32_t row0 = mb * kTile + g * kRows, col0 = kb * kTile + c * 8;
-    const int left = int(P.k) - int(col0);
+    const uint32_t tiles = P.k_blocks * P.m_blocks;
 
-    float v[kRows][8];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        if (row0 + r < P.m && left > 0) {
-            load8<T, VEC>(static_cast<const T *>(P.x) + size_t(row0 + r) * P.ld + col0, left, v[r]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][i] = 0.0f;
-        }
-    }
-    if (TURNED && P.sums) {
-        // column sums of the tile, rows in a fixed order
-        float sum[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            sum[i] = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
-            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
-        }
-        float *sums = reinterpret_cast<float *>(tile);  // [kWarps][kTile]
-        if (lane < 16) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<float4 *>(sums + warp * kTile + c * 8 + i) =
-                    make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
-        }
-        __syncthreads();
-        if (threadIdx.x < kTile && kb * kTile + threadIdx.x < P.k) {
-            float s = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) s += sums[w * kTile + threadIdx.x];
-            P.sums[size_t(mb) * P.k + kb * kTile + threadIdx.x] = s;
-        }
-        __syncthreads();
-    }
-    // infinities become NaN, which the maxima below pass over (0 * v is 0
-    // for every finite v, so most threads find none)
-    float any = 0.0f;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) any = fmaf(v[r][i], 0.0f, any);
-    if (any != 0.0f) {
-#pragma unroll
-        for (int r = 0; r < kRows; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (fabsf(v[r][i]) == __int_as_float(0x7f800000)) v[r][i] = __int_as_float(0x7fc00000);
-    }
-
-    uint32_t whole = 127;  // scale exponent of the 128 x 128 block
-    if (BLOCK_ROWS == 128) {
-        float top = 0.0f;
-#pragma unroll
-        for (int r = 0; r < kRows; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[r][i]));
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-        if (lane == 0) top_all[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, top_all[w]);
-        whole = scale_exponent(top);
-        if (threadIdx.x == 0) {
-            if (NORMAL) P.scales[size_t(kb) * P.m_blocks + mb] = scale_value(whole);
-            if (TURNED) P.turned_scales[size_t(mb) * P.k_blocks + kb] = scale_value(whole);
-        }
-    }
-    if (TURNED && BLOCK_ROWS == 1) {
-        float top[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            top[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
-            top[i] = fmaxf(0.0f, top[i]);  // four NaN
-            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-        }
-        if (lane < 16) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<float4 *>(&tops[warp][c * 8 + i]) = make_float4(top[i], top[i + 1], top[i + 2], top[i + 3]);
-        }
-        __syncthreads();
-        if (threadIdx.x < kTile) {
-            float t = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) t = fmaxf(t, tops[w][threadIdx.x]);
-            const uint32_t e = scale_exponent(t), col = kb * kTile + threadIdx.x;
-            inverses[threadIdx.x] = scale_inverse(e);
-            if (col < P.k) P.turned_scales[size_t(mb) * P.k + col] = scale_value(e);
-        }
-    }
-
-    if (NORMAL) {
+    auto prefetch = [&](uint32_t t, uint32_t buffer) {
+        const uint32_t kb = t % P.k_blocks, mb = t / P.k_blocks;
+        const uint32_t row = mb * kTile + g * kRows, col = kb * kTile + c * 8;
+        unsigned char *dst = staged + ((buffer * kTile + g * kRows) * kTile + c * 8) * sizeof(T);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-            uint32_t exponent = whole;
-            if (BLOCK_ROWS == 1) {
-                float top = 0.0f;
+            const bool in = row + r < P.m && col < P.k;
+            const T *src = static_cast<const T *>(P.x) + (in ? size_t(row + r) * P.ld + col : 0);
+            stage8<T>(dst + r * kTile * sizeof(T), src, in ? int(min(P.k - col, 8u)) : 0);
+        }
+    };
+    if (VEC) {
+        if (blockIdx.x < tiles) prefetch(blockIdx.x, 0);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    uint32_t buffer = 0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, buffer ^= 1) {
+        const uint32_t kb = t % P.k_blocks, mb = t / P.k_blocks;
+        const uint32_t row0 = mb * kTile + g * kRows, col0 = kb * kTile + c * 8;
+        const int left = int(P.k) - int(col0);
+
+        float v[kRows][8];
+        if (VEC) {
+            if (t + gridDim.x < tiles) prefetch(t + gridDim.x, buffer ^ 1);
+            asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+            const unsigned char *src = staged + ((buffer * kTile + g * kRows) * kTile + c * 8) * sizeof(T);
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                union Eight {
+                    uint4 q[sizeof(T) / 2];
+                    T e[8];
+                    __device__ Eight() {}
+                } u;
+#pragma unroll
+                for (int i = 0; i < int(sizeof(T) / 2); ++i)
+                    u.q[i] = *reinterpret_cast<const uint4 *>(src + r * kTile * sizeof(T) + 16 * i);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[r][i] = as_float(u.e[i]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const T *src = static_cast<const T *>(P.x) + size_t(row0 + r) * P.ld + col0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[r][i] = row0 + r < P.m && i < left ? as_float(src[i]) : 0.0f;
+            }
+        }
+        if (TURNED && P.sums) {
+            // column sums of the tile, rows in a fixed order
+            float sum[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum[i] = (v[0][i] + v[1][i]) + (v[2][i] + v[3][i]);
+                sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+            }
+            float *sums = reinterpret_cast<float *>(tile);  // [kWarps][kTile]
+            if (lane < 16) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 4)
+                    *reinterpret_cast<float4 *>(sums + warp * kTile + c * 8 + i) =
+                        make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+            }
+            __syncthreads();
+            if (threadIdx.x < kTile && kb * kTile + threadIdx.x < P.k) {
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) s += sums[w * kTile + threadIdx.x];
+                P.sums[size_t(mb) * P.k + kb * kTile + threadIdx.x] = s;
+            }
+            __syncthreads();
+        }
+        // infinities become NaN, which the maxima below pass over (0 * v is 0
+        // for every finite v, so most threads find none)
+        float any = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) any = fmaf(v[r][i], 0.0f, any);
+        if (any != 0.0f) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (fabsf(v[r][i]) == __int_as_float(0x7f800000)) v[r][i] = __int_as_float(0x7fc00000);
+        }
+
+        uint32_t whole = 127;  // scale exponent of the 128 x 128 block
+        if (BLOCK_ROWS == 128) {
+            float top = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[r][i]));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            if (lane == 0) top_all[warp] = top;
+            __syncthreads();
 #pragma unroll
-                for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                exponent = scale_exponent(top);
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, top_all[w]);
+            whole = scale_exponent(top);
+            if (threadIdx.x == 0) {
+                if (NORMAL) P.scales[size_t(kb) * P.m_blocks + mb] = scale_value(whole);
+                if (TURNED) P.turned_scales[size_t(mb) * P.k_blocks + kb] = scale_value(whole);
             }
-            const float inv = scale_inverse(exponent);
-            if (row0 + r < P.m) {
-                if (BLOCK_ROWS == 1 && c == 0) P.scales[size_t(kb) * P.m + row0 + r] = scale_value(exponent);
-                // whole 16-byte pieces of the row are written, zeros past k
-                if (col0 < ((P.k + 15u) & ~15u)) {
-                    uint2 q;
-                    q.x = pack4(v[r][0] * inv, v[r][1] * inv, v[r][2] * inv, v[r][3] * inv);
-                    q.y = pack4(v[r][4] * inv, v[r][5] * inv, v[r][6] * inv, v[r][7] * inv);
-                    *reinterpret_cast<uint2 *>(P.values + size_t(row0 + r) * P.ldv + col0) = q;
+        }
+        if (TURNED && BLOCK_ROWS == 1) {
+            float top[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                top[i] = fmaxf(fmaxf(fabsf(v[0][i]), fabsf(v[1][i])), fmaxf(fabsf(v[2][i]), fabsf(v[3][i])));
+                top[i] = fmaxf(0.0f, top[i]);  // four NaN
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+            }
+            if (lane < 16) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 4)
+                    *reinterpret_cast<float4 *>(&tops[warp][c * 8 + i]) = make_float4(top[i], top[i + 1], top[i + 2], top[i + 3]);
+            }
+            __syncthreads();
+            if (threadIdx.x < kTile) {
+                float t = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) t = fmaxf(t, tops[w][threadIdx.x]);
+                const uint32_t e = scale_exponent(t), col = kb * kTile + threadIdx.x;
+                inverses[threadIdx.x] = scale_inverse(e);
+                if (col < P.k) P.turned_scales[size_t(mb) * P.k + col] = scale_value(e);
+            }
+        }
+
+        if (NORMAL) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                uint32_t exponent = whole;
+                if (BLOCK_ROWS == 1) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[r][i]));
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    exponent = scale_exponent(top);
+                }
+                const float inv = scale_inverse(exponent);
+                if (row0 + r < P.m) {
+                    if (BLOCK_ROWS == 1 && c == 0) P.scales[size_t(kb) * P.m + row0 + r] = scale_value(exponent);
+                    // whole 16-byte pieces of the row are written, zeros past k
+                    if (col0 < ((P.k + 15u) & ~15u)) {
+                        uint2 q;
+                        q.x = pack4(v[r][0] * inv, v[r][1] * inv, v[r][2] * inv, v[r][3] * inv);
+                        q.y = pack4(v[r][4] * inv, v[r][5] * inv, v[r][6] * inv, v[r][7] * inv);
+                        *reinterpret_cast<uint2 *>(P.values + size_t(row0 + r) * P.ldv + col0) = q;
+                    }
                 }
             }
         }
-    }
 
-    if (TURNED) {
-        float inv[8];
-        if (BLOCK_ROWS == 1) {
-            __syncthreads();
+        if (TURNED) {
+            float inv[8];
+            if (BLOCK_ROWS == 1) {
+                __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const float4 q = *reinterpret_cast<const float4 *>(&inverses[c * 8 + i]);
-                inv[i] = q.x;
-                inv[i + 1] = q.y;
-                inv[i + 2] = q.z;
-                inv[i + 3] = q.w;
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(&inverses[c * 8 + i]);
+                    inv[i] = q.x;
+                    inv[i + 1] = q.y;
+                    inv[i + 2] = q.z;
+                    inv[i + 3] = q.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) inv[i] = scale_inverse(whole);
             }
-        } else {
+            // column j of the tile: 32 words of 4 rows, word g at place
+            // g ^ 2 (j / 8), so that the lanes of a store fall on different banks
 #pragma unroll
-            for (int i = 0; i < 8; ++i) inv[i] = scale_inverse(whole);
+            for (int i = 0; i < 8; ++i)
+                tile[(c * 8 + i) * 32 + (g ^ (2 * c))] = pack4(v[0][i] * inv[i], v[1][i] * inv[i], v[2][i] * inv[i], v[3][i] * inv[i]);
+            __syncthreads();
+            // 16 bytes per thread and turn: whole 16-byte pieces of the turned
+            // rows, zeros past m
+            const uint32_t m16 = (P.m + 15u) & ~15u;
+#pragma unroll
+            for (int i = 0; i < int(kTile * 8 / kThreads); ++i) {
+                const uint32_t at = i * kThreads + threadIdx.x, j = at >> 3, s = at & 7, turn = (j >> 3) & 15;
+                uint4 q = *reinterpret_cast<const uint4 *>(tile + j * 32 + ((s ^ (turn >> 1)) << 2));
+                if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
+                const uint32_t row = kb * kTile + j, col = mb * kTile + 16 * s;
+                if (row < P.k && col < m16) *reinterpret_cast<uint4 *>(P.turned + size_t(row) * P.ldt + col) = q;
+            }
         }
-        // column j of the tile: 32 words of 4 rows, word g at place
-        // g ^ 2 (j / 8), so that the lanes of a store fall on different banks
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            tile[(c * 8 + i) * 32 + (g ^ (2 * c))] = pack4(v[0][i] * inv[i], v[1][i] * inv[i], v[2][i] * inv[i], v[3][i] * inv[i]);
-        __syncthreads();
-        // 16 bytes per thread and turn: whole 16-byte pieces of the turned
-        // rows, zeros past m
-        const uint32_t m16 = (P.m + 15u) & ~15u;
-#pragma unroll
-        for (int t = 0; t < int(kTile * 8 / kThreads); ++t) {
-            const uint32_t at = t * kThreads + threadIdx.x, j = at >> 3, s = at & 7, turn = (j >> 3) & 15;
-            uint4 q = *reinterpret_cast<const uint4 *>(tile + j * 32 + ((s ^ (turn >> 1)) << 2));
-            if (turn & 1) q = make_uint4(q.z, q.w, q.x, q.y);
-            const uint32_t row = kb * kTile + j, col = mb * kTile + 16 * s;
-            if (row < P.k && col < m16) *reinterpret_cast<uint4 *>(P.turned + size_t(row) * P.ldt + col) = q;
-        }
+        if (TURNED || BLOCK_ROWS == 128) __syncthreads();  // the next tile takes the shared memory
     }
 }
 
@@ -349,20 +386,32 @@ __global__ void __launch_bounds__(kDequantThreads) dequantize_kernel(const unsig
     }
 }
 
+template <typename T, bool VEC, int BLOCK_ROWS, bool NORMAL, bool TURNED>
+cudaError_t quantize_launch(const QuantParams &P, cudaStream_t stream) {
+    auto kernel = quantize_kernel<T, VEC, BLOCK_ROWS, NORMAL, TURNED>;
+    constexpr size_t kStaged = VEC ? 2 * kTile * kTile * sizeof(T) : 0;
+    // two blocks of an SM where their staging fits, one for fp32
+    constexpr unsigned kResident = sizeof(T) == 4 && VEC ? 148 : 2 * 148;
+    if (kStaged > 0) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kStaged));
+        if (e != cudaSuccess) return e;
+    }
+    kernel<<<std::min(P.k_blocks * P.m_blocks, kResident), kThreads, kStaged, stream>>>(P);
+    return cudaGetLastError();
+}
+
 template <typename T, bool VEC, int BLOCK_ROWS>
-void quantize_out(const QuantParams &P, unsigned blocks, cudaStream_t stream) {
-    if (P.values && P.turned) quantize_kernel<T, VEC, BLOCK_ROWS, true, true><<<blocks, kThreads, 0, stream>>>(P);
-    else if (P.values) quantize_kernel<T, VEC, BLOCK_ROWS, true, false><<<blocks, kThreads, 0, stream>>>(P);
-    else quantize_kernel<T, VEC, BLOCK_ROWS, false, true><<<blocks, kThreads, 0, stream>>>(P);
+cudaError_t quantize_out(const QuantParams &P, cudaStream_t stream) {
+    if (P.values && P.turned) return quantize_launch<T, VEC, BLOCK_ROWS, true, true>(P, stream);
+    if (P.values) return quantize_launch<T, VEC, BLOCK_ROWS, true, false>(P, stream);
+    return quantize_launch<T, VEC, BLOCK_ROWS, false, true>(P, stream);
 }
 
 template <typename T>
-void quantize_typed(const QuantParams &P, int block_rows, unsigned blocks, cudaStream_t stream) {
+cudaError_t quantize_typed(const QuantParams &P, int block_rows, cudaStream_t stream) {
     const bool vec = ((reinterpret_cast<uintptr_t>(P.x) | (P.ld * sizeof(T))) & 15u) == 0;
-    if (vec && block_rows == 1) quantize_out<T, true, 1>(P, blocks, stream);
-    else if (vec) quantize_out<T, true, 128>(P, blocks, stream);
-    else if (block_rows == 1) quantize_out<T, false, 1>(P, blocks, stream);
-    else quantize_out<T, false, 128>(P, blocks, stream);
+    if (vec) return block_rows == 1 ? quantize_out<T, true, 1>(P, stream) : quantize_out<T, true, 128>(P, stream);
+    return block_rows == 1 ? quantize_out<T, false, 1>(P, stream) : quantize_out<T, false, 128>(P, stream);
 }
 
 template <typename T>
@@ -399,13 +448,9 @@ cudaError_t launch_block_quantize(const void *x, size_t ld, uint32_t dtype, uint
     P.sums = column_sums ? sums : nullptr;
     P.k_blocks = (k + kTile - 1) / kTile;
     P.m_blocks = (m + kTile - 1) / kTile;
-    const unsigned blocks = P.k_blocks * P.m_blocks;
-    switch (dtype) {
-        case SDFOAM_F32: quantize_typed<float>(P, block_rows, blocks, stream); break;
-        case SDFOAM_F16: quantize_typed<__half>(P, block_rows, blocks, stream); break;
-        default: quantize_typed<__nv_bfloat16>(P, block_rows, blocks, stream); break;
-    }
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = dtype == SDFOAM_F32   ? quantize_typed<float>(P, block_rows, stream)
+                          : dtype == SDFOAM_F16 ? quantize_typed<__half>(P, block_rows, stream)
+                                                : quantize_typed<__nv_bfloat16>(P, block_rows, stream);
     if (e != cudaSuccess || !column_sums) return e;
     const unsigned columns = (k + 31) / 32;
     switch (sums_dtype) {
