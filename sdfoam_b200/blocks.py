@@ -13,6 +13,8 @@ gradients are 8-bit products of operands quantized on the way.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -111,7 +113,7 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1, transpose: bool = Fals
     if block_rows not in (1, _BLOCK):
         raise RuntimeError("block_rows must be 1 or 128")
     _cuda("x", x)
-    return _quantize(x.detach(), block_rows, bool(transpose))
+    return _quantize(x, block_rows, bool(transpose))
 
 
 def _block_rows(what: str, values: torch.Tensor, scales: torch.Tensor) -> int:
@@ -122,10 +124,12 @@ def _block_rows(what: str, values: torch.Tensor, scales: torch.Tensor) -> int:
     if scales.dtype != torch.float32:
         raise RuntimeError(f"the scales of {what} must have float32 dtype")
     m, k = values.shape
-    if tuple(scales.shape) == (m, _blocks(k)):
-        return 1
-    if tuple(scales.shape) == (_blocks(m), _blocks(k)):
-        return _BLOCK
+    rows, columns = scales.shape
+    if columns == _blocks(k):
+        if rows == m:
+            return 1
+        if rows == _blocks(m):
+            return _BLOCK
     raise RuntimeError(f"the scales of {what} must have shape [{m} or {_blocks(m)}, {_blocks(k)}]")
 
 
@@ -148,40 +152,22 @@ def dequantize_blocks(values: torch.Tensor, scales: torch.Tensor, dtype: torch.d
     return out
 
 
-def _operand(v: torch.Tensor) -> torch.Tensor:
-    """Rows 16 bytes aligned, as the copies into shared memory need them."""
-    m, k = v.shape
-    if v.stride(1) == 1 and v.stride(0) >= k and v.stride(0) % 16 == 0 and v.data_ptr() % 16 == 0:
-        return v
-    out = _values(m, k, v.device)
+def _operand(v: torch.Tensor):
+    """(v, bytes between its rows): rows 16 bytes aligned, as the copies into
+    shared memory need them."""
+    rows, step = v.stride()
+    k = v.shape[1]
+    if step == 1 and rows >= k and rows % 16 == 0 and v.data_ptr() % 16 == 0:
+        return v, rows
+    out = _values(v.shape[0], k, v.device)
     out.copy_(v)
-    return out
-
-
-def _product(a, a_scales, a_rows, b, b_scales, b_rows, bias, out_dtype):
-    a, b = _operand(a), _operand(b)
-    m, k = a.shape
-    n = b.shape[0]
-    dev = a.device
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    lib = _lib.load()
-    nbytes = lib.sdfoam_block_matmul_workspace_bytes(m, n, k)
-    with _lib.on(dev):
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(lib.sdfoam_block_matmul(
-            a.data_ptr(), max(a.stride(0), k), a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), a_rows, m,
-            b.data_ptr(), max(b.stride(0), k), b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), b_rows,
-            n, k, None if bias is None else bias.data_ptr(),
-            0 if bias is None else _DTYPES[bias.dtype], out.data_ptr(), max(n, 1), _DTYPES[out_dtype],
-            None if ws is None else ws.data_ptr(), nbytes, _flag(dev), _lib.stream(dev)))
-    return out
+    return out, max(out.stride(0), k)
 
 
 def _check_bias(bias, n, device):
-    if bias is not None:
-        if bias.dtype not in _DTYPES or tuple(bias.shape) != (n,):
-            raise RuntimeError(f"bias must be a float32, float16 or bfloat16 vector of {n}")
-        _cuda("bias", bias, device)
+    if bias.dtype not in _DTYPES or bias.dim() != 1 or bias.shape[0] != n:
+        raise RuntimeError(f"bias must be a float32, float16 or bfloat16 vector of {n}")
+    _cuda("bias", bias, device)
 
 
 def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
@@ -193,16 +179,34 @@ def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
     see :func:`block_linear`."""
     a_rows = _block_rows("a", a, a_scales)
     b_rows = _block_rows("b", b, b_scales)
-    if a.shape[1] != b.shape[1]:
-        raise RuntimeError(f"a and b must have the same number of columns, got {a.shape[1]} and {b.shape[1]}")
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        raise RuntimeError(f"a and b must have the same number of columns, got {k} and {b.shape[1]}")
     if out_dtype not in _DTYPES:
         raise RuntimeError("out_dtype must be float32, float16 or bfloat16")
-    _cuda("a", a)
-    for what, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
-        _cuda(what, t, a.device)
-    _check_bias(bias, b.shape[0], a.device)
-    bias = None if bias is None else bias.detach().contiguous()
-    return _product(a, a_scales.detach(), a_rows, b, b_scales.detach(), b_rows, bias, out_dtype)
+    dev = a.device
+    if dev.type != "cuda" or a_scales.device != dev or b.device != dev or b_scales.device != dev:
+        _cuda("a", a)
+        for what, t in (("a_scales", a_scales), ("b", b), ("b_scales", b_scales)):
+            _cuda(what, t, dev)
+    if bias is not None:
+        _check_bias(bias, n, dev)
+        bias = bias.contiguous()
+    lib = _lib.load()
+    nbytes = lib.sdfoam_block_matmul_workspace_bytes(m, n, k)
+    with _lib.on(dev):
+        a, lda = _operand(a)
+        b, ldb = _operand(b)
+        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.check(lib.sdfoam_block_matmul(
+            a.data_ptr(), lda, a_scales.data_ptr(), *a_scales.stride(), a_rows, m,
+            b.data_ptr(), ldb, b_scales.data_ptr(), *b_scales.stride(), b_rows, n, k,
+            None if bias is None else bias.data_ptr(), 0 if bias is None else _DTYPES[bias.dtype],
+            out.data_ptr(), max(n, 1), _DTYPES[out_dtype], None if ws is None else ws.data_ptr(), nbytes, _flag(dev),
+            _lib.stream(dev)))
+    return out
 
 
 class _BlockLinear(torch.autograd.Function):
@@ -280,9 +284,9 @@ def block_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
             raise RuntimeError(f"{what} must have float32, float16 or bfloat16 dtype")
     _cuda("x", x)
     _cuda("weight", weight, x.device)
-    _check_bias(bias, weight.shape[0], x.device)
-    rows = 1
-    for d in x.shape[:-1]:
-        rows *= d
-    y = _BlockLinear.apply(x.reshape(rows, x.shape[-1]), weight, bias)
+    if bias is not None:
+        _check_bias(bias, weight.shape[0], x.device)
+    if x.dim() == 2:
+        return _BlockLinear.apply(x, weight, bias)
+    y = _BlockLinear.apply(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]), weight, bias)
     return y.reshape(*x.shape[:-1], weight.shape[0])

@@ -26,8 +26,10 @@
 // unless a has few rows (a single token to 64): then a's rows are the narrow
 // side, so that a weight is read once with 128 of its rows per tile and TN
 // columns of tokens.  When the tiles do not fill the GPU, the reduction is
-// cut into slices; their fp32 sums go to the workspace and a second launch
-// adds them in order (no atomics: the same bits every run).
+// cut into slices, whose fp32 sums are added in order (no atomics: the same
+// bits every run): up to 8 slices of a narrow tile are a cluster that adds
+// them through its shared memory, otherwise they go to the workspace and a
+// second launch adds them.
 //
 // Every wait is bounded: a CTA that gives up sets *error, writes NaN, waits
 // (bounded) for its own copies and MMAs and frees its TMEM.  No TMA multicast.
@@ -94,6 +96,7 @@ struct BlockParams {
     uint32_t out_dtype;
     int store;
     float4 *parts;                     // splits > 1: sums of the slices
+    int cluster_join;                  // splits > 1: a tile's slices are a cluster, joined in it
     int *error;
 };
 
@@ -405,6 +408,27 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
     }
 }
 
+// Float4 number i of a tile's sums (the order of its CTAs' epilogues), plus
+// the bias, to its four places of out.
+template <int TN, bool SWAP, bool PAIR>
+__device__ __forceinline__ void store_four(const BlockParams &P, const Unit &t, uint32_t i, const float (&v)[4]) {
+    using S = Shape<TN, PAIR>;
+    constexpr int kCols = S::kCols;
+    constexpr uint32_t kPerCta = kTileP * TN / 4;
+    const uint32_t rank = i / kPerCta, in = i % kPerCta;
+    // warp w of the epilogue: quarter w % 4, group w / 4
+    const uint32_t lane = in & 31, c4 = (in >> 5) % (kCols / 4), w = (in >> 5) / (kCols / 4);
+    const uint32_t row = (t.tp * S::kCtas + rank) * kTileP + (w & 3) * 32 + lane;
+    const uint32_t col = t.tq * TN + (w / 4) * kCols + c4 * 4;
+    if (row >= P.p_rows) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= P.q_rows) return;
+        const uint32_t n = SWAP ? row : col + e, m = SWAP ? col + e : row;
+        store_value(P.out, P.out_dtype, uint64_t(m) * P.ldo + n, P.bias ? v[e] + bias_at(P, n) : v[e]);
+    }
+}
+
 // QROWS: a scale per row of Q (per column of the tile) instead of one per 128.
 // SWAP: P is b and Q is a; the tile is stored turned.
 // PAIR: two CTAs share a tile of 256 rows of P; each brings its 128 rows and
@@ -419,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
     using S = Shape<TN, PAIR>;
     constexpr int kCols = S::kCols;
     constexpr int kChunk = 8;
+    constexpr uint32_t kPart = kTileP * TN / 4;  // float4 of a CTA's sums: [warp][columns / 4][lane]
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char *boxes = smem + S::kStages * S::kStageBytes;
@@ -644,7 +669,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
             }
             if (P.splits > 1) {
                 const size_t block = PAIR ? size_t(u) * 2 + rank : u;
-                float4 *dst = P.parts + ((block * kEpiWarps + (warp - 4)) * (kCols / 4)) * 32 + lane;
+                // in a cluster: over the operands' ring, which is done with
+                float4 *dst = TN <= 64 && P.cluster_join ? reinterpret_cast<float4 *>(smem) : P.parts + block * kPart;
+                dst += (warp - 4) * (kCols / 4) * 32 + lane;
 #pragma unroll
                 for (int i = 0; i < kCols / 4; ++i) {
                     const float2 x = unpair(acc[2 * i]), y = unpair(acc[2 * i + 1]);
@@ -682,6 +709,36 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
         *static_cast<volatile int *>(P.error) = 1;
         __threadfence_system();
     }
+    if constexpr (TN <= 64 && !PAIR) {
+        if (P.cluster_join) {
+            // one unit per CTA: the slices of a tile, each CTA adds its share
+            // of them in order
+            cluster_sync();
+            const Unit t = unit_of(P, blockIdx.x);
+            const uint32_t own = cluster_rank(), mine = smem_u32(smem);
+            for (uint32_t i = own * kThreads + threadIdx.x; i < kPart; i += P.splits * kThreads) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t s = 0; s < P.splits; ++s) {
+                    float4 x;
+                    asm volatile(
+                        "{\n"
+                        ".reg .b32 a;\n"
+                        "mapa.shared::cluster.u32 a, %4, %5;\n"
+                        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n"
+                        "}\n"
+                        : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                        : "r"(mine + i * 16), "r"(s)
+                        : "memory");
+                    v[0] += x.x;
+                    v[1] += x.y;
+                    v[2] += x.z;
+                    v[3] += x.w;
+                }
+                store_four<TN, SWAP, PAIR>(P, t, i, v);
+            }
+            cluster_sync();  // the others have read this CTA's sums
+        }
+    }
     // the other CTA's copies, commits and arrivals are done before either leaves
     if constexpr (PAIR) cluster_sync();
     if (warp == 1) {
@@ -695,18 +752,13 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
 }
 
 // Adds the slices of a tile in order (parts: [tile][slice][CTA][warp]
-// [columns / 4][lane] float4, the epilogue's own order) and the bias.
+// [columns / 4][lane] float4) and the bias.
 template <int TN, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(256) join_slices_kernel(const BlockParams P) {
-    using S = Shape<TN, PAIR>;
-    constexpr int kCols = S::kCols, kCtas = S::kCtas;
-    constexpr uint32_t kPerCta = kEpiWarps * (kCols / 4) * 32, kPerTile = kPerCta * kCtas;
+    constexpr uint32_t kPerTile = kTileP * TN / 4 * Shape<TN, PAIR>::kCtas;
     const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
     const uint32_t tile = uint32_t(i / kPerTile), in = uint32_t(i % kPerTile);
     if (tile >= P.tiles_p * P.tiles_q) return;
-    const uint32_t rank = in / kPerCta;
-    const uint32_t lane = in & 31, c4 = (in >> 5) % (kCols / 4), w = (in % kPerCta >> 5) / (kCols / 4);
-    const Unit t = unit_of(P, tile * P.splits);
     const float4 *src = P.parts + size_t(tile) * P.splits * kPerTile + in;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -717,16 +769,7 @@ __global__ void __launch_bounds__(256) join_slices_kernel(const BlockParams P) {
         v[2] += x.z;
         v[3] += x.w;
     }
-    const uint32_t row = (t.tp * kCtas + rank) * kTileP + (w & 3) * 32 + lane;  // warp w of the epilogue: quarter w % 4, group w / 4
-    const uint32_t col = t.tq * TN + (w / 4) * kCols + c4 * 4;
-    if (row >= P.p_rows) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (col + e >= P.q_rows) return;
-        const uint32_t n = SWAP ? row : col + e, m = SWAP ? col + e : row;
-        if (P.bias) v[e] += bias_at(P, n);
-        store_value(P.out, P.out_dtype, uint64_t(m) * P.ldo + n, v[e]);
-    }
+    store_four<TN, SWAP, PAIR>(P, unit_of(P, tile * P.splits), in, v);
 }
 
 // The bias (or zero) everywhere: a product over nothing.
@@ -742,7 +785,7 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(const BlockParams P, uin
 // --------------------------------------------------------------------------
 
 struct Plan {
-    bool swap, pair;
+    bool swap, pair, cluster_join;
     int tn;
     uint32_t tiles_p, tiles_q, k_blocks, splits;
 };
@@ -761,6 +804,11 @@ Plan plan_of(uint32_t m, uint32_t n, uint32_t k) {
     l.pair = l.tn == 256;
     if (l.pair) l.tiles_p = (l.tiles_p + 1) / 2;
     l.splits = !l.pair && tiles < kSms ? std::min<uint32_t>(l.k_blocks, uint32_t(kSms / tiles)) : 1;
+    // narrow tiles: a cluster of up to 8 slices (the portable size), and no
+    // more slices where 16 blocks or fewer are left to each: a second launch
+    // costs about as much as 8 blocks
+    if (l.tn <= 64 && l.splits > 8 && l.k_blocks <= 128) l.splits = 8;
+    l.cluster_join = l.tn <= 64 && l.splits > 1 && l.splits <= 8;
     return l;
 }
 
@@ -808,11 +856,11 @@ cudaError_t launch_tiles(const CUtensorMap &mp, const CUtensorMap &mq, const CUt
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S::kCtas;
+    attr[0].val.clusterDim.x = PAIR ? 2 : P.splits;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    if ((e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, mo, P)) != cudaSuccess || P.splits == 1) return e;
+    cfg.numAttrs = PAIR || P.cluster_join ? 1 : 0;
+    if ((e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, mo, P)) != cudaSuccess || P.splits == 1 || P.cluster_join) return e;
     const uint64_t threads = uint64_t(P.tiles_p) * P.tiles_q * S::kCtas * kTileP * TN / 4;
     join_slices_kernel<TN, SWAP, PAIR><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(P);
     return cudaGetLastError();
@@ -840,7 +888,7 @@ cudaError_t launch_tn(const Plan &l, const CUtensorMap &mp, const CUtensorMap &m
 size_t block_matmul_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
     if (m == 0 || n == 0 || k == 0) return 0;
     const Plan l = plan_of(m, n, k);
-    return l.splits > 1 ? size_t(l.tiles_p) * l.tiles_q * l.splits * (l.pair ? 2 : 1) * kTileP * l.tn * 4 : 0;
+    return l.splits > 1 && !l.cluster_join ? size_t(l.tiles_p) * l.tiles_q * l.splits * (l.pair ? 2 : 1) * kTileP * l.tn * 4 : 0;
 }
 
 cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
@@ -876,6 +924,7 @@ cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scal
     P.p_shift = (l.swap ? b_block_rows : a_block_rows) == 128 ? 7 : 0;
     P.q_shift = (l.swap ? a_block_rows : b_block_rows) == 128 ? 7 : 0;
     P.parts = static_cast<float4 *>(workspace);
+    P.cluster_join = l.cluster_join;
     P.error = error;
     const uint32_t size = out_dtype == SDFOAM_F32 ? 4 : 2;
     const uintptr_t at = reinterpret_cast<uintptr_t>(out);
