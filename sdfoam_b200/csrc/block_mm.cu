@@ -69,10 +69,12 @@ struct Shape {
     static constexpr int kGroups = 2, kCols = TN / kGroups;  // groups of four epilogue warps, their columns
     // per epilogue warp: its 32 rows x kCols columns of 16 bits, at least a box of 32 x 128 bytes
     static constexpr uint32_t kBoxBytes = kCols < 32 ? 0 : kCols == 128 ? 8192 : 4096;
-    static constexpr int kScaleStages = 6;
+    static constexpr int kScaleStages = 8;
     static constexpr uint32_t kScaleFloats = kTileP + TN;  // of a block: P's rows, Q's rows
     static constexpr uint32_t kSmem =
         kStages * kStageBytes + kEpiWarps * kBoxBytes + (kScaleStages * kScaleFloats + TN) * 4 + 512 + 1024;
+    static_assert(kSmem <= 232448, "shared memory of a block");
+    static_assert((2 * kStages + 2 * kAccs + 2 * kScaleStages + 1) * 8 + 4 <= 512, "room for the barriers");
 };
 
 // How a tile's rows reach out.
@@ -408,17 +410,14 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
     }
 }
 
-// Float4 number i of a tile's sums (the order of its CTAs' epilogues), plus
-// the bias, to its four places of out.
-template <int TN, bool SWAP, bool PAIR>
+// Float4 number i of a tile's sums (the epilogue's order), plus the bias, to
+// its four places of out.
+template <int TN, bool SWAP>
 __device__ __forceinline__ void store_four(const BlockParams &P, const Unit &t, uint32_t i, const float (&v)[4]) {
-    using S = Shape<TN, PAIR>;
-    constexpr int kCols = S::kCols;
-    constexpr uint32_t kPerCta = kTileP * TN / 4;
-    const uint32_t rank = i / kPerCta, in = i % kPerCta;
+    constexpr int kCols = Shape<TN, false>::kCols;
     // warp w of the epilogue: quarter w % 4, group w / 4
-    const uint32_t lane = in & 31, c4 = (in >> 5) % (kCols / 4), w = (in >> 5) / (kCols / 4);
-    const uint32_t row = (t.tp * S::kCtas + rank) * kTileP + (w & 3) * 32 + lane;
+    const uint32_t lane = i & 31, c4 = (i >> 5) % (kCols / 4), w = (i >> 5) / (kCols / 4);
+    const uint32_t row = t.tp * kTileP + (w & 3) * 32 + lane;
     const uint32_t col = t.tq * TN + (w / 4) * kCols + c4 * 4;
     if (row >= P.p_rows) return;
 #pragma unroll
@@ -667,10 +666,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
 #pragma unroll
                 for (int i = 0; i < kCols / 2; ++i) acc[i] = 0x7fc000007fc00000ull;
             }
-            if (P.splits > 1) {
-                const size_t block = PAIR ? size_t(u) * 2 + rank : u;
+            if (!PAIR && P.splits > 1) {
                 // in a cluster: over the operands' ring, which is done with
-                float4 *dst = TN <= 64 && P.cluster_join ? reinterpret_cast<float4 *>(smem) : P.parts + block * kPart;
+                float4 *dst = TN <= 64 && P.cluster_join ? reinterpret_cast<float4 *>(smem) : P.parts + size_t(u) * kPart;
                 dst += (warp - 4) * (kCols / 4) * 32 + lane;
 #pragma unroll
                 for (int i = 0; i < kCols / 4; ++i) {
@@ -690,8 +688,21 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                 }
             } else if constexpr (kCols >= 32) {
                 store_rows<kCols, S::kGroups>(P, &map_out, stage, row_stage, acc, row0, col0, lane, group, quarter);
+            } else if (row < P.p_rows && P.out_dtype != SDFOAM_F32 && col0 + kCols <= P.q_rows &&
+                       ((reinterpret_cast<uintptr_t>(P.out) | (P.ldo * 2)) & 15u) == 0) {
+                // 8 or 16 columns per thread, 16 bytes at a time
+                uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(P.out) + uint64_t(row) * P.ldo + col0);
+#pragma unroll
+                for (int q = 0; q < kCols / 8; ++q) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 x = unpair(acc[q * 4 + e]);
+                        w[e] = pack2(P.out_dtype, x.x, x.y);
+                    }
+                    dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             } else if (row < P.p_rows) {
-                // at most 16 columns per thread
 #pragma unroll
                 for (int i = 0; i < kCols / 2; ++i) {
                     const float2 x = unpair(acc[i]);
@@ -734,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                     v[2] += x.z;
                     v[3] += x.w;
                 }
-                store_four<TN, SWAP, PAIR>(P, t, i, v);
+                store_four<TN, SWAP>(P, t, i, v);
             }
             cluster_sync();  // the others have read this CTA's sums
         }
@@ -751,25 +762,54 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
     }
 }
 
-// Adds the slices of a tile in order (parts: [tile][slice][CTA][warp]
-// [columns / 4][lane] float4) and the bias.
-template <int TN, bool SWAP, bool PAIR>
-__global__ void __launch_bounds__(256) join_slices_kernel(const BlockParams P) {
-    constexpr uint32_t kPerTile = kTileP * TN / 4 * Shape<TN, PAIR>::kCtas;
-    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
-    const uint32_t tile = uint32_t(i / kPerTile), in = uint32_t(i % kPerTile);
-    if (tile >= P.tiles_p * P.tiles_q) return;
-    const float4 *src = P.parts + size_t(tile) * P.splits * kPerTile + in;
+// Adds the slices of a tile in order (parts: [tile][slice][warp][columns / 4]
+// [lane] float4) and the bias.  A block takes the 32 rows x kCols columns of
+// one epilogue warp, or 16 columns of them where there are MANY slices, read
+// as that warp wrote them: groups of threads take consecutive runs of the
+// slices, their sums are added in order and turned in shared memory, so that
+// consecutive threads store consecutive elements (512 x 2048 of two slices:
+// 12 us stored straight from the parts' order, 4.7 so; 256 x 256 of 37: 7.5
+// and 3.5).
+constexpr int kJoinThreads = 512;
+
+template <int TN, bool MANY>
+constexpr int join_columns() {
+    return MANY && Shape<TN, false>::kCols > 16 ? 16 : Shape<TN, false>::kCols;
+}
+
+template <int TN, bool SWAP, bool MANY>
+__global__ void __launch_bounds__(kJoinThreads) join_slices_kernel(const BlockParams P) {
+    constexpr int kCols = Shape<TN, false>::kCols, kTake = join_columns<TN, MANY>(), kPieces = kCols / kTake;
+    constexpr uint32_t kPerTile = kTileP * TN / 4, kItems = kTake / 4 * 32, kRuns = kJoinThreads / kItems;
+    __shared__ float sums[kRuns][32][kTake + 1];
+    const uint32_t piece = blockIdx.x % kPieces, w = blockIdx.x / kPieces % kEpiWarps, tile = blockIdx.x / (kPieces * kEpiWarps);
+    const uint32_t run = threadIdx.x / kItems, i = threadIdx.x % kItems;
+    const float4 *src = P.parts + size_t(tile) * P.splits * kPerTile + (w * kPieces + piece) * kItems + i;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t s1 = (run + 1) * P.splits / kRuns;
 #pragma unroll 4
-    for (uint32_t s = 0; s < P.splits; ++s) {
+    for (uint32_t s = run * P.splits / kRuns; s < s1; ++s) {
         const float4 x = __ldcs(src + size_t(s) * kPerTile);
         v[0] += x.x;
         v[1] += x.y;
         v[2] += x.z;
         v[3] += x.w;
     }
-    store_four<TN, SWAP, PAIR>(P, unit_of(P, tile * P.splits), in, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[run][i & 31][(i >> 5) * 4 + e] = v[e];
+    __syncthreads();
+    const Unit t = unit_of(P, tile * P.splits);
+    const uint32_t row0 = t.tp * kTileP + (w & 3) * 32, col0 = t.tq * TN + (w / 4) * kCols + piece * kTake;
+    for (uint32_t o = threadIdx.x; o < 32 * kTake; o += kJoinThreads) {
+        const uint32_t r = SWAP ? o % 32 : o / kTake, c = SWAP ? o / 32 : o % kTake;
+        const uint32_t row = row0 + r, col = col0 + c;
+        if (row >= P.p_rows || col >= P.q_rows) continue;
+        const uint32_t n = SWAP ? row : col, m = SWAP ? col : row;
+        float x = sums[0][r][c];
+#pragma unroll
+        for (uint32_t q = 1; q < kRuns; ++q) x += sums[q][r][c];
+        store_value(P.out, P.out_dtype, uint64_t(m) * P.ldo + n, P.bias ? x + bias_at(P, n) : x);
+    }
 }
 
 // The bias (or zero) everywhere: a product over nothing.
@@ -861,8 +901,13 @@ cudaError_t launch_tiles(const CUtensorMap &mp, const CUtensorMap &mq, const CUt
     cfg.attrs = attr;
     cfg.numAttrs = PAIR || P.cluster_join ? 1 : 0;
     if ((e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, mo, P)) != cudaSuccess || P.splits == 1 || P.cluster_join) return e;
-    const uint64_t threads = uint64_t(P.tiles_p) * P.tiles_q * S::kCtas * kTileP * TN / 4;
-    join_slices_kernel<TN, SWAP, PAIR><<<unsigned((threads + 255) / 256), 256, 0, stream>>>(P);
+    if constexpr (!PAIR) {
+        const unsigned warps = P.tiles_p * P.tiles_q * kEpiWarps;
+        if (P.splits > 8)
+            join_slices_kernel<TN, SWAP, true><<<warps * (S::kCols / join_columns<TN, true>()), kJoinThreads, 0, stream>>>(P);
+        else
+            join_slices_kernel<TN, SWAP, false><<<warps, kJoinThreads, 0, stream>>>(P);
+    }
     return cudaGetLastError();
 }
 
