@@ -152,14 +152,21 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 // counts the digits of each tile, scans the counts, and scatters: every warp
 // ranks its 256 consecutive entries by ballots over the digit's bits and its
 // own digit counts (__match_any_sync took 360 cycles a call here), the tile is put in order in shared memory and leaves in runs of
-// equal digits.  The first pass reads the ids themselves.  Up to 8192 entries
-// are sorted by one block in one launch.
+// equal digits.  The first pass reads the ids themselves.
+//
+// Launches count where there are few ids.  Up to 64 tiles need no scan: every
+// block adds up the counts of the tiles before its own, and a pass counts the
+// next one's digits while it writes (integer atomics: the same counts in any
+// order).  Up to 8192 entries are sorted by one block in one launch (4097: the
+// same time on the GPU as five launches, 8 us less with the call).
 
 constexpr int kSortThreads = 256;
 constexpr int kSortItems = 8;
 constexpr uint32_t kSortTile = kSortThreads * kSortItems;
 constexpr int kMaxBins = 512;
 constexpr uint32_t kBlockSort = 8192;  // entries that one block sorts
+constexpr uint32_t kFewTiles = 64;
+constexpr int kMaxPasses = 4;          // 32 bits by 9
 
 uint32_t sort_tiles(uint32_t n) { return (n + kSortTile - 1) / kSortTile; }
 
@@ -167,7 +174,10 @@ struct SortPass {
     const void *ids;               // the first pass's input
     const uint32_t *keys_in, *vals_in;
     uint32_t *keys_out, *vals_out;
-    uint32_t *counts;              // [bins][tiles], then its exclusive scan along the tiles
+    uint32_t *counts;              // [bins][tiles], then its exclusive scan along the tiles;
+                                   // few tiles: [tiles][bins]
+    uint32_t *next_counts;         // few tiles: the next pass's, or null
+    uint32_t clear_counts;         // few tiles, first pass: words behind counts that later passes add to
     uint32_t *totals;              // [bins]
     uint32_t n, rows, tiles;
     int shift, bins;
@@ -187,11 +197,14 @@ __device__ __forceinline__ void clear_touched(unsigned char *touched, uint32_t r
         reinterpret_cast<uint4 *>(touched)[w] = make_uint4(0, 0, 0, 0);
 }
 
-template <typename I, bool FIRST>
+template <typename I, bool FIRST, bool FEW>
 __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const SortPass P) {
     __shared__ uint32_t count[kMaxBins];
     for (int b = threadIdx.x; b < P.bins; b += kSortThreads) count[b] = 0;
     if (FIRST) clear_touched(P.touched, P.rows, blockIdx.x, gridDim.x);
+    if (FEW)
+        for (uint32_t w = blockIdx.x * kSortThreads + threadIdx.x; w < P.clear_counts; w += gridDim.x * kSortThreads)
+            P.counts[P.tiles * P.bins + w] = 0;
     __syncthreads();
     const uint32_t base = blockIdx.x * kSortTile, mask = P.bins - 1;
 #pragma unroll
@@ -200,7 +213,8 @@ __global__ void __launch_bounds__(kSortThreads) digit_counts_kernel(const SortPa
         if (i < P.n) atomicAdd(&count[(sort_key<I, FIRST>(P, i) >> P.shift) & mask], 1u);
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < P.bins; b += kSortThreads) P.counts[size_t(b) * P.tiles + blockIdx.x] = count[b];
+    for (int b = threadIdx.x; b < P.bins; b += kSortThreads)
+        P.counts[FEW ? blockIdx.x * P.bins + b : size_t(b) * P.tiles + blockIdx.x] = count[b];
 }
 
 // Exclusive scan of each digit's counts along the tiles, one warp per digit.
@@ -309,7 +323,7 @@ __device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint
         if (digit[r] < uint32_t(bins)) rank[r] += mine[digit[r]] + start[digit[r]];
 }
 
-template <typename I, bool FIRST>
+template <typename I, bool FIRST, bool FEW>
 __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const SortPass P) {
     constexpr int kWarps = kSortThreads / 32;
     __shared__ uint32_t keys[kSortTile];
@@ -335,7 +349,20 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
     uint32_t carry = 0;
     for (int b0 = 0; b0 < P.bins; b0 += kSortThreads) {
         const int b = b0 + int(threadIdx.x);
-        const uint32_t total = b < P.bins ? P.totals[b] : 0u;
+        uint32_t total = 0, earlier = 0;
+        if (b < P.bins) {
+            if (FEW) {
+#pragma unroll 8
+                for (uint32_t t = 0; t < P.tiles; ++t) {
+                    const uint32_t x = P.counts[t * P.bins + b];
+                    total += x;
+                    if (t < blockIdx.x) earlier += x;
+                }
+            } else {
+                total = P.totals[b];
+                earlier = P.counts[size_t(b) * P.tiles + blockIdx.x];
+            }
+        }
         uint32_t incl = total;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -350,7 +377,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
             if (uint32_t(w) < warp) before += warp_sums[w];
             all += warp_sums[w];
         }
-        if (b < P.bins) base[b] = before + incl - total + P.counts[size_t(b) * P.tiles + blockIdx.x] - start[b];
+        if (b < P.bins) base[b] = before + incl - total + earlier - start[b];
         carry += all;
         __syncthreads();
     }
@@ -360,7 +387,11 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < valid; i += kSortThreads) {
         const uint32_t k = keys[i], at = base[(k >> P.shift) & mask] + i;
-        if (at < P.n) P.keys_out[at] = k;  // always, for consistent counts; keeps the store in bounds
+        if (at < P.n) {  // always, for consistent counts; keeps the store in bounds
+            P.keys_out[at] = k;
+            if (FEW && P.next_counts)
+                atomicAdd(P.next_counts + at / kSortTile * P.bins + ((k >> P.shift) / P.bins & mask), 1u);
+        }
     }
     // the values, in the order of their keys (the counts are no longer needed)
 #pragma unroll
@@ -379,18 +410,20 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
 // clear the rows' marks.
 constexpr int kBlockSortThreads = 1024;
 constexpr int kBlockSortBins = 256;
-constexpr size_t kBlockSortSmem = kBlockSort * 8 + kBlockSortThreads / 32 * kBlockSortBins * 2 + kBlockSortBins * 4 + 128;
+constexpr size_t block_sort_smem(int items) {
+    return size_t(kBlockSortThreads) * items * 8 + kBlockSortThreads / 32 * kBlockSortBins * 2 + kBlockSortBins * 4 + 128;
+}
 
-template <typename I>
+template <typename I, int kItems>
 __global__ void __launch_bounds__(kBlockSortThreads) sort_block_kernel(const SortPass P, int bits) {
     extern __shared__ __align__(16) unsigned char raw[];
     if (blockIdx.x > 0) {
         clear_touched(P.touched, P.rows, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
-    constexpr int kWarps = kBlockSortThreads / 32, kItems = kBlockSort / kBlockSortThreads;
-    uint32_t *keys = reinterpret_cast<uint32_t *>(raw), *vals = keys + kBlockSort;
-    uint16_t *counts = reinterpret_cast<uint16_t *>(vals + kBlockSort);
+    constexpr int kWarps = kBlockSortThreads / 32;
+    uint32_t *keys = reinterpret_cast<uint32_t *>(raw), *vals = keys + kBlockSortThreads * kItems;
+    uint16_t *counts = reinterpret_cast<uint16_t *>(vals + kBlockSortThreads * kItems);
     uint32_t *start = reinterpret_cast<uint32_t *>(counts + kWarps * kBlockSortBins), *warp_sums = start + kBlockSortBins;
     const uint32_t first = (threadIdx.x >> 5) * (32 * kItems) + (threadIdx.x & 31);
     uint32_t key[kItems], val[kItems], digit[kItems], rank[kItems];
@@ -703,7 +736,7 @@ RowGradLayout grad_layout(uint32_t n, uint32_t rows, uint32_t columns) {
         l.keys[i] = take(size_t(n) * 4);
         l.vals[i] = take(size_t(n) * 4);
     }
-    l.counts = take(size_t(kMaxBins) * sort_tiles(n) * 4);
+    l.counts = take(size_t(kMaxBins) * sort_tiles(n) * 4 * (sort_tiles(n) <= kFewTiles ? kMaxPasses : 1));
     l.totals = take(kMaxBins * 4);
     l.touched = take(rows);
     l.chunk = chunk_of(n);
@@ -773,8 +806,18 @@ cudaError_t sum_typed(SumParams &P, cudaStream_t stream) {
     else sum_rows_kernel<T, VB, 1><<<grid, kSumThreads, 0, stream>>>(P);
     P.join_blocks = (P.chunks + kJoinWarps - 1) / kJoinWarps;
     const uint64_t zero_units = uint64_t(P.rows) * P.units;
-    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 4095) / 4096, 148 * 4));
+    const uint32_t zero_blocks = uint32_t(std::min<uint64_t>((zero_units + 4095) / 4096, 148 * 16));
     join_parts_kernel<T, VB><<<P.join_blocks + zero_blocks, kJoinThreads, 0, stream>>>(P);
+    return cudaGetLastError();
+}
+
+template <typename I, int ITEMS>
+cudaError_t sort_in_block(const SortPass &P, int bits, cudaStream_t stream) {
+    constexpr size_t kSmem = block_sort_smem(ITEMS);
+    cudaError_t e = cudaFuncSetAttribute(sort_block_kernel<I, ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
+    if (e != cudaSuccess) return e;
+    const unsigned clear = unsigned(std::min<uint64_t>((uint64_t(P.rows) + 16383) / 16384, 147));
+    sort_block_kernel<I, ITEMS><<<1 + clear, kBlockSortThreads, kSmem, stream>>>(P, bits);
     return cudaGetLastError();
 }
 
@@ -783,19 +826,18 @@ cudaError_t sort_ids(SortPass &P, uint32_t *const keys[2], uint32_t *const vals[
     int bits = 0;  // of the largest key, `rows`
     while (bits < 32 && (uint64_t(P.rows) >> bits) != 0) ++bits;
     if (P.n <= kBlockSort) {
-        cudaError_t e = cudaFuncSetAttribute(sort_block_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             int(kBlockSortSmem));
-        if (e != cudaSuccess) return e;
         cur = 0;
         P.keys_out = keys[0];
         P.vals_out = vals[0];
-        const unsigned clear = unsigned(std::min<uint64_t>((uint64_t(P.rows) + 16383) / 16384, 147));
-        sort_block_kernel<I><<<1 + clear, kBlockSortThreads, kBlockSortSmem, stream>>>(P, bits);
-        return cudaGetLastError();
+        return P.n <= 2 * kBlockSortThreads ? sort_in_block<I, 2>(P, bits, stream)
+                                            : sort_in_block<I, kBlockSort / kBlockSortThreads>(P, bits, stream);
     }
     const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes;
     P.tiles = sort_tiles(P.n);
     P.bins = 1 << width;
+    const bool few = P.tiles <= kFewTiles;
+    const uint32_t words = P.tiles * P.bins;
+    uint32_t *const counts = P.counts;
     cur = 0;
     for (int p = 0; p < passes; ++p) {
         P.shift = p * width;
@@ -803,11 +845,20 @@ cudaError_t sort_ids(SortPass &P, uint32_t *const keys[2], uint32_t *const vals[
         P.vals_in = vals[cur ^ 1];
         P.keys_out = keys[cur];
         P.vals_out = vals[cur];
-        if (p == 0) digit_counts_kernel<I, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
-        else digit_counts_kernel<I, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
-        scan_counts_kernel<<<(P.bins + 7) / 8, 256, 0, stream>>>(P);
-        if (p == 0) scatter_digits_kernel<I, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
-        else scatter_digits_kernel<I, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        if (few) {
+            P.clear_counts = (passes - 1) * words;
+            if (p == 0) digit_counts_kernel<I, true, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
+            P.counts = counts + p * words;
+            P.next_counts = p + 1 < passes ? P.counts + words : nullptr;
+            if (p == 0) scatter_digits_kernel<I, true, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
+            else scatter_digits_kernel<I, false, true><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        } else {
+            if (p == 0) digit_counts_kernel<I, true, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+            else digit_counts_kernel<I, false, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+            scan_counts_kernel<<<(P.bins + 7) / 8, 256, 0, stream>>>(P);
+            if (p == 0) scatter_digits_kernel<I, true, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+            else scatter_digits_kernel<I, false, false><<<P.tiles, kSortThreads, 0, stream>>>(P);
+        }
         if (p + 1 < passes) cur ^= 1;
     }
     return cudaGetLastError();

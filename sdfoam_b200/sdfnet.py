@@ -25,6 +25,11 @@ gradient is a tcgen05 GEMM reducing over the rows with both operands
 MN-major (sdfoam_mlp_wgrad), and the encoding's gradient a tcgen05 GEMM with
 the skip connection's gradient added in its epilogue (sdfoam_mlp_input_grad).
 Other shapes and the CPU use the plain PyTorch layers below.
+
+`dtype=torch.float8_e4m3fn` keeps float32 weights and bf16 activations and
+runs every linear layer as an 8-bit product (blocks.block_linear: e4m3 with a
+scale per block of 128, forward and both gradients), for networks wide enough
+that the products' rate counts; any width and depth, CUDA only.
 """
 from __future__ import annotations
 
@@ -34,6 +39,8 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .blocks import block_linear
 
 
 def positional_encoding(x: torch.Tensor, multires: int) -> torch.Tensor:
@@ -52,6 +59,8 @@ class WeightNormLinear(nn.Module):
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor, dtype):
         super().__init__()
+        if dtype == torch.float8_e4m3fn:
+            dtype = torch.float32  # quantized on the way into each product
         v = weight.detach().clone()
         g = v.norm(dim=1, keepdim=True)
         self.weight_g = nn.Parameter(g.to(dtype))
@@ -111,7 +120,7 @@ class SDFNetwork(nn.Module):
             if weight_norm:
                 lin = WeightNormLinear(w, b, dtype)
             else:
-                lin = nn.Linear(dims[l], out_dim, dtype=dtype)
+                lin = nn.Linear(dims[l], out_dim, dtype=torch.float32 if dtype == torch.float8_e4m3fn else dtype)
                 with torch.no_grad():
                     lin.weight.copy_(w)
                     lin.bias.copy_(b)
@@ -133,19 +142,24 @@ class SDFNetwork(nn.Module):
         return self.forward_layers(inputs)
 
     def forward_layers(self, inputs: torch.Tensor) -> torch.Tensor:
-        """The network as plain PyTorch layers (sdfnet.py:120-136)."""
+        """The network as plain PyTorch layers (sdfnet.py:120-136); with dtype
+        float8_e4m3fn their products in 8 bits."""
+        eight = self.dtype == torch.float8_e4m3fn
         if self.pc_center is not None:
             inputs = inputs - self.pc_center
         inputs = inputs * self.scale
         if self.multires > 0:
             inputs = positional_encoding(inputs, self.multires)
-        inputs = inputs.to(self.dtype)
+        inputs = inputs.to(torch.bfloat16 if eight else self.dtype)
         x = inputs
         for l in range(self.num_layers - 1):
             lin = getattr(self, f"lin{l}")
             if l in self.skip_in:
                 x = torch.cat([x, inputs], 1) / math.sqrt(2.0)
-            x = lin(x)
+            if eight:
+                x = block_linear(x, lin.weight() if self.weight_norm else lin.weight, lin.bias)
+            else:
+                x = lin(x)
             if l < self.num_layers - 2:
                 x = F.softplus(x, beta=100)
         x = x.float()
@@ -164,6 +178,9 @@ class SDFNetwork(nn.Module):
         loss is differentiated, its double backward on the library's tcgen05
         kernels.  Otherwise the plain PyTorch layers, whose double backward
         autograd provides."""
+        if self.dtype == torch.float8_e4m3fn:
+            raise RuntimeError("8-bit layers have no second derivative; take input gradients for the eikonal term "
+                               "with dtype=torch.bfloat16 or torch.float32")
         x = x.requires_grad_(True)
         if self.fused_ok(x):
             return FusedSDFGradient.apply(x.float().contiguous(), self.pc_center, float(self.scale),

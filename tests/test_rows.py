@@ -103,9 +103,10 @@ def test_lookup_shapes_and_strides():
 @pytest.mark.parametrize("columns", [1, 2, 3, 49, 256, 700])
 def test_gradient(dtype, columns):
     g = torch.Generator(device="cuda").manual_seed(columns)
-    # one block sorts up to 8192 ids; more take passes of up to 9 bits
+    # one block sorts up to 8192 ids; more take passes of up to 9 bits, in
+    # tiles of 2048 whose counts are scanned by a launch of its own past 64
     for n, rows in ((1, 1), (5, 300), (127, 5), (1000, 70000), (4097, 256), (8192, 65536), (8193, 1), (20000, 255),
-                    (20000, 512), (30011, 66000), (9000, 300000)):
+                    (20000, 512), (30011, 66000), (9000, 300000), (131072, 511), (131073, 90000)):
         v = torch.randint(-2, rows + 2, (n,), generator=g, device="cuda")
         grad = torch.randn((n, columns), generator=g, device="cuda").to(dtype)
         for index in (torch.uint32, torch.int64):
