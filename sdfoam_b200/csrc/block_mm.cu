@@ -81,7 +81,7 @@ struct Shape {
 enum : int {
     kStoreRows,  // element by element, consecutive lanes on consecutive columns
     kStoreBox,   // TMA boxes of 32 rows x 128 bytes: rows of out are 16-byte aligned
-    kStoreSpan,  // one tile covers whole contiguous rows: 32 rows are one bulk copy
+    kStoreSpan,  // one tile covers whole contiguous rows, both groups: 32 rows are one bulk copy
 };
 
 struct BlockParams {
@@ -274,29 +274,43 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
     // this warp's previous stores have read the buffer
     if (P.store != kStoreRows && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     if (P.store == kStoreSpan) {
-        // 16-bit rows of q_rows columns one after another, all groups
-        asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
-        const uint32_t n = P.q_rows, left = n - min(n, col0), odd = (lane * n + col0) & 1u;
-        uint16_t *dst = reinterpret_cast<uint16_t *>(row_stage) + lane * n + col0;
-        // whole words: a row that starts on half a word stores its first
-        // column alone and the pairs one column further
-        uint32_t w = 0, before = 0;
+        // 16-bit rows of q_rows columns one after another: kCols < q_rows <= 2
+        // kCols.  The second group stores all its columns, past its rows'
+        // ends into the next rows' first columns; the first group's, which
+        // are all in the row, come after it (bounds for each column instead
+        // of the order: 260 us for 1M x 217 x 256, 161 so).  Whole words: a
+        // row that starts on half a word stores its first column alone, then
+        // the pairs of columns 2 i - 1 and 2 i, then its last.
+        const uint32_t n = P.q_rows, odd = (lane * n + group * kCols) & 1u;
+        uint16_t *dst = reinterpret_cast<uint16_t *>(row_stage) + lane * n + group * kCols;
+        uint32_t w[kCols / 2 + 1];
+        w[0] = 0;
 #pragma unroll
-        for (int i = 0; i <= kCols / 2; ++i) {
-            if (i < kCols / 2) {
-                const float2 x = unpair(acc[i]);
-                w = pack2(P.out_dtype, x.x, x.y);
-            }
-            // columns c and c + 1: 2 i and 2 i + 1, or 2 i - 1 and 2 i
-            const uint32_t pair = odd ? __byte_perm(before, w, 0x5432) : w;
-            const int c = 2 * i - int(odd);
-            if (i < kCols / 2 && c >= 0 && uint32_t(c) + 1 < left) {
-                *reinterpret_cast<uint32_t *>(dst + c) = pair;
+        for (int i = 0; i < kCols / 2; ++i) {
+            const float2 x = unpair(acc[i]);
+            w[i + 1] = pack2(P.out_dtype, x.x, x.y);
+        }
+        const uint16_t head = uint16_t(w[1]), tail = uint16_t(w[kCols / 2] >> 16);
+        if (odd) {
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) w[i] = __byte_perm(w[i], w[i + 1], 0x5432);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) w[i] = w[i + 1];
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
+#pragma unroll
+        for (uint32_t turn = 0; turn < uint32_t(kGroups); ++turn) {
+            if (turn > 0) asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
+            if (group == turn) continue;
+            if (odd) {
+                dst[0] = head;
+                dst[kCols - 1] = tail;
             } else {
-                if (c >= 0 && uint32_t(c) < left && c < kCols) dst[c] = uint16_t(pair);
-                if (i < kCols / 2 && c < 0 && left > 0) dst[0] = uint16_t(pair >> 16);
+                *reinterpret_cast<uint32_t *>(dst) = w[0];
             }
-            before = w;
+#pragma unroll
+            for (int i = 1; i < kCols / 2; ++i) *reinterpret_cast<uint32_t *>(dst + 2 * i - odd) = w[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
@@ -975,7 +989,7 @@ cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scal
     const uintptr_t at = reinterpret_cast<uintptr_t>(out);
     P.store = l.tn < 64 || l.swap || l.splits > 1                   ? kStoreRows
               : ((at | (ldo * size)) & 15u) == 0                   ? kStoreBox
-              : size == 2 && l.tiles_q == 1 && ldo == n && !(at & 15u) ? kStoreSpan
+              : size == 2 && l.tiles_q == 1 && n > uint32_t(l.tn) / 2 && ldo == n && !(at & 15u) ? kStoreSpan
                                                                    : kStoreRows;
     CUtensorMap mp, mq, mo{};
     if (!operand_map(&mp, l.swap ? b : a, P.p_rows, k, l.swap ? ldb : lda, kTileP) ||
