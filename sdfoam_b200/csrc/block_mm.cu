@@ -194,6 +194,13 @@ __device__ __forceinline__ void tmem_load(uint32_t (&r)[8], uint32_t addr) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
         : "r"(addr));
 }
+// 16 lanes x 16 columns: thread t holds columns 2 (t % 4) and + 1 of rows t / 4
+// (r[0], r[1]) and t / 4 + 8 (r[2], r[3]), and of the columns 8 further (r[4..7]).
+__device__ __forceinline__ void tmem_load_patch(uint32_t (&r)[8], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+}
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
     asm volatile(
         "tcgen05.wait::ld.sync.aligned;"
@@ -266,14 +273,16 @@ __device__ __forceinline__ Unit unit_of(const BlockParams &P, uint32_t u) {
 // `stage` is the warp's staging buffer, `row_stage` that of the warps of its
 // rows.  Rows go to shared memory in pieces of 16 bytes, swizzled as the TMA
 // unit (or the element-wise reader) expects: piece q of row r of a box of 128
-// bytes at q ^ (r & 7), of 64 bytes at q ^ ((r / 2) & 3).
-template <int kCols, int kGroups>
+// bytes at q ^ (r & 7), of 64 bytes at q ^ ((r / 2) & 3).  PATCH: the thread
+// holds columns 2 (lane % 4) and + 1 of each 8 (cg) of rows 8 j + lane / 4, at
+// acc[4 cg + j].
+template <int kCols, int kGroups, bool PATCH>
 __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorMap *map, unsigned char *stage,
                                            unsigned char *row_stage, const uint64_t (&acc)[kCols / 2], uint32_t row0,
                                            uint32_t col0, uint32_t lane, uint32_t group, uint32_t quarter) {
     // this warp's previous stores have read the buffer
     if (P.store != kStoreRows && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    if (P.store == kStoreSpan) {
+    if (!PATCH && P.store == kStoreSpan) {
         // 16-bit rows of q_rows columns one after another: kCols < q_rows <= 2
         // kCols.  The second group stores all its columns, past its rows'
         // ends into the next rows' first columns; the first group's, which
@@ -334,8 +343,21 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
     constexpr int kBoxes16 = kCols / kCols16, kBoxes32 = kCols / 32, kFit32 = kBoxes32 >= 2 ? kBoxes32 / 2 : 1;
     const uint32_t sw16 = kCols16 == 64 ? (lane & 7u) : ((lane >> 1) & 3u);
     if (!wide) {
+        if constexpr (PATCH) {
+            static_assert(kCols16 == 64, "a patch stores boxes of 128 bytes");
 #pragma unroll
-        for (int b = 0; b < kBoxes16; ++b) {
+            for (int cg = 0; cg < kCols / 8; ++cg) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = unpair(acc[4 * cg + j]);
+                    unsigned char *row = stage + cg / 8 * 4096 + (8 * j + (lane >> 2)) * 128;
+                    *reinterpret_cast<uint32_t *>(row + (((cg % 8) ^ (lane >> 2)) << 4) + (lane & 3u) * 4) =
+                        pack2(P.out_dtype, x.x, x.y);
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < (PATCH ? 0 : kBoxes16); ++b) {
             unsigned char *box = stage + b * (32 * kCols16 * 2) + lane * (kCols16 * 2);
 #pragma unroll
             for (int q = 0; q < kCols16 / 8; ++q) {
@@ -388,9 +410,19 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
         }
 #pragma unroll
         for (int b = b0; b < b0 + kFit32; ++b) {
+            if constexpr (PATCH) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int cg = i / 4, j = i % 4;  // of the box's 32 columns
+                    const float2 x = unpair(acc[16 * b + 4 * cg + j]);
+                    unsigned char *row = stage + (b - b0) * 4096 + (8 * j + (lane >> 2)) * 128;
+                    const uint32_t q = 2 * cg + ((lane & 3u) >> 1);
+                    *reinterpret_cast<float2 *>(row + ((q ^ (lane >> 2)) << 4) + (lane & 1u) * 8) = x;
+                }
+            }
             unsigned char *box = stage + (b - b0) * 4096 + lane * 128;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < (PATCH ? 0 : 8); ++q) {
                 const float2 x = unpair(acc[b * 16 + q * 2]), y = unpair(acc[b * 16 + q * 2 + 1]);
                 *reinterpret_cast<float4 *>(box + ((q ^ (lane & 7u)) << 4)) = make_float4(x.x, x.y, y.x, y.y);
             }
@@ -456,6 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
     using S = Shape<TN, PAIR>;
     constexpr int kCols = S::kCols;
     constexpr int kChunk = 8;
+    // A scale per column is a value per column for every thread that holds one
+    // row: at 128 bytes a cycle shared memory takes twice the MMAs' time to
+    // hand them out (4096^3: 111 us, 75 without those reads).  Where the tile is
+    // wide, a thread holds 4 rows of a quarter of the columns instead.
+    constexpr bool kPatch = QROWS && !SWAP && TN >= 128;
     constexpr uint32_t kPart = kTileP * TN / 4;  // float4 of a CTA's sums: [warp][columns / 4][lane]
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -633,8 +670,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                     bias_tq = t.tq;
                 }
 #pragma unroll
-                for (int i = 0; i < kCols / 2; ++i)
-                    acc[i] = *reinterpret_cast<const uint64_t *>(bias_s + group * kCols + 2 * i);
+                for (int i = 0; i < kCols / 2; ++i) {
+                    const int column = kPatch ? i / 4 * 8 + int(lane & 3u) * 2 : 2 * i;
+                    acc[i] = *reinterpret_cast<const uint64_t *>(bias_s + group * kCols + column);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
@@ -645,28 +684,58 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                 if (!mbar_wait(scale_full + 8 * ss, (done / S::kScaleStages) & 1, &abort_flag)) bad = true;
                 const float *sc = scales + ss * S::kScaleFloats;
                 const float *q_sc = sc + kTileP + (QROWS ? group * kCols : group);
-                const float one = QROWS ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * *q_sc;
+                float one = 0.0f;
+                uint64_t p4[kPatch ? 4 : 1];
+                if constexpr (kPatch) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = sc[quarter * 32 + 8 * j + (lane >> 2)];
+                        p4[j] = pair(p, p);
+                    }
+                } else {
+                    one = QROWS ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * *q_sc;
+                }
                 if (!mbar_wait(acc_full + 8 * b, turn & 1, &abort_flag)) bad = true;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
-                const uint64_t s2 = pair(one, one);
+                if constexpr (kPatch) {
 #pragma unroll
-                for (int c = 0; c < kCols / kChunk; ++c) {
-                    uint32_t v[kChunk];
-                    tmem_load(v, addr + c * kChunk);
-                    tmem_wait(v);
+                    for (int c = 0; c < kCols / 16; ++c) {
+                        const uint64_t *qp = reinterpret_cast<const uint64_t *>(q_sc + c * 16 + (lane & 3u) * 2);
+                        const uint64_t q2[2] = {qp[0], qp[4]};
 #pragma unroll
-                    for (int i = 0; i < kChunk; i += 4) {
-                        const uint64_t x = pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                        const uint64_t y = pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-                        uint64_t sx = s2, sy = s2;
-                        if (QROWS) {
-                            const float4 q = *reinterpret_cast<const float4 *>(q_sc + c * kChunk + i);
-                            sx = mul_pair(s2, pair(q.x, q.y));
-                            sy = mul_pair(s2, pair(q.z, q.w));
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t v[8];
+                            tmem_load_patch(v, addr + (uint32_t(16 * h) << 16) + c * 16);
+                            tmem_wait(v);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int g = i / 2, j = 2 * h + i % 2;
+                                const uint64_t x = pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                                fma_pair(acc[4 * (2 * c + g) + j], x, mul_pair(p4[j], q2[g]));
+                            }
                         }
-                        fma_pair(acc[(c * kChunk + i) / 2], x, sx);
-                        fma_pair(acc[(c * kChunk + i) / 2 + 1], y, sy);
+                    }
+                } else {
+                    const uint64_t s2 = pair(one, one);
+#pragma unroll
+                    for (int c = 0; c < kCols / kChunk; ++c) {
+                        uint32_t v[kChunk];
+                        tmem_load(v, addr + c * kChunk);
+                        tmem_wait(v);
+#pragma unroll
+                        for (int i = 0; i < kChunk; i += 4) {
+                            const uint64_t x = pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                            const uint64_t y = pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                            uint64_t sx = s2, sy = s2;
+                            if (QROWS) {
+                                const float4 q = *reinterpret_cast<const float4 *>(q_sc + c * kChunk + i);
+                                sx = mul_pair(s2, pair(q.x, q.y));
+                                sy = mul_pair(s2, pair(q.z, q.w));
+                            }
+                            fma_pair(acc[(c * kChunk + i) / 2], x, sx);
+                            fma_pair(acc[(c * kChunk + i) / 2 + 1], y, sy);
+                        }
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;");
@@ -683,11 +752,20 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
             if (!PAIR && P.splits > 1) {
                 // in a cluster: over the operands' ring, which is done with
                 float4 *dst = TN <= 64 && P.cluster_join ? reinterpret_cast<float4 *>(smem) : P.parts + size_t(u) * kPart;
-                dst += (warp - 4) * (kCols / 4) * 32 + lane;
+                dst += (warp - 4) * (kCols / 4) * 32;
+                if constexpr (kPatch) {
 #pragma unroll
-                for (int i = 0; i < kCols / 4; ++i) {
-                    const float2 x = unpair(acc[2 * i]), y = unpair(acc[2 * i + 1]);
-                    dst[i * 32] = make_float4(x.x, x.y, y.x, y.y);
+                    for (int i = 0; i < kCols / 2; ++i) {
+                        const int c4 = i / 4 * 2, j = i % 4;
+                        float4 *at = dst + (c4 + ((lane & 3u) >> 1)) * 32 + 8 * j + (lane >> 2);
+                        reinterpret_cast<float2 *>(at)[lane & 1u] = unpair(acc[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kCols / 4; ++i) {
+                        const float2 x = unpair(acc[2 * i]), y = unpair(acc[2 * i + 1]);
+                        dst[i * 32 + lane] = make_float4(x.x, x.y, y.x, y.y);
+                    }
                 }
             } else if constexpr (SWAP) {
                 // lane = column of out: the warp writes 32 consecutive elements
@@ -701,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                         store_value(P.out, P.out_dtype, uint64_t(col0 + 2 * i + 1) * P.ldo + row, x.y + bias);
                 }
             } else if constexpr (kCols >= 32) {
-                store_rows<kCols, S::kGroups>(P, &map_out, stage, row_stage, acc, row0, col0, lane, group, quarter);
+                store_rows<kCols, S::kGroups, kPatch>(P, &map_out, stage, row_stage, acc, row0, col0, lane, group, quarter);
             } else if (row < P.p_rows && P.out_dtype != SDFOAM_F32 && col0 + kCols <= P.q_rows &&
                        ((reinterpret_cast<uintptr_t>(P.out) | (P.ldo * 2)) & 15u) == 0) {
                 // 8 or 16 columns per thread, 16 bytes at a time
@@ -989,7 +1067,7 @@ cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scal
     const uintptr_t at = reinterpret_cast<uintptr_t>(out);
     P.store = l.tn < 64 || l.swap || l.splits > 1                   ? kStoreRows
               : ((at | (ldo * size)) & 15u) == 0                   ? kStoreBox
-              : size == 2 && l.tiles_q == 1 && n > uint32_t(l.tn) / 2 && ldo == n && !(at & 15u) ? kStoreSpan
+              : size == 2 && l.tiles_q == 1 && P.q_shift != 0 && n > uint32_t(l.tn) / 2 && ldo == n && !(at & 15u) ? kStoreSpan
                                                                    : kStoreRows;
     CUtensorMap mp, mq, mo{};
     if (!operand_map(&mp, l.swap ? b : a, P.p_rows, k, l.swap ? ldb : lda, kTileP) ||
