@@ -906,10 +906,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_slices_kernel(const BlockPa
 
 // The bias (or zero) everywhere: a product over nothing.
 __global__ void __launch_bounds__(256) fill_bias_kernel(const BlockParams P, uint32_t m, uint32_t n) {
-    const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= uint64_t(m) * n) return;
-    const uint32_t r = uint32_t(i / n), c = uint32_t(i % n);
-    store_value(P.out, P.out_dtype, uint64_t(r) * P.ldo + c, P.bias ? bias_at(P, c) : 0.0f);
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < uint64_t(m) * n; i += uint64_t(gridDim.x) * 256) {
+        const uint32_t r = uint32_t(i / n), c = uint32_t(i % n);
+        store_value(P.out, P.out_dtype, uint64_t(r) * P.ldo + c, P.bias ? bias_at(P, c) : 0.0f);
+    }
 }
 
 // --------------------------------------------------------------------------
@@ -1041,7 +1041,7 @@ cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scal
     P.ldo = ldo;
     P.out_dtype = out_dtype;
     if (k == 0) {
-        fill_bias_kernel<<<unsigned((uint64_t(m) * n + 255) / 256), 256, 0, stream>>>(P, m, n);
+        fill_bias_kernel<<<unsigned(std::min<uint64_t>((uint64_t(m) * n + 255) / 256, kSms * 32)), 256, 0, stream>>>(P, m, n);
         return cudaGetLastError();
     }
     const Plan l = plan_of(m, n, k);

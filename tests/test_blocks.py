@@ -290,6 +290,65 @@ def test_linear_shapes_and_parts():
 
 
 @pytest.mark.gpu
+def test_linear_over_nothing():
+    """No columns to sum over, no outputs, an empty batch."""
+    bias = torch.randn(4, device="cuda", requires_grad=True)
+    x = torch.randn((5, 0), device="cuda", requires_grad=True)
+    w = torch.randn((4, 0), device="cuda", requires_grad=True)
+    y = foam.block_linear(x, w, bias)
+    assert torch.equal(y, bias.expand(5, 4))
+    gx, gw, gb = torch.autograd.grad(y.sum(), (x, w, bias))
+    assert gx.shape == (5, 0) and gw.shape == (4, 0) and torch.equal(gb, torch.full((4,), 5.0, device="cuda"))
+    x = torch.randn((5, 6), device="cuda", requires_grad=True)
+    w = torch.randn((0, 6), device="cuda", requires_grad=True)
+    y = foam.block_linear(x, w)
+    assert y.shape == (5, 0)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert (gx == 0).all() and gw.shape == (0, 6)
+    for transpose in (False, True):
+        v, s = foam.quantize_blocks(torch.zeros((0, 5), device="cuda"), transpose=transpose)
+        assert foam.dequantize_blocks(v, s).shape == ((5, 0) if transpose else (0, 5))
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads_and_streams():
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((300, 256), generator=g, device="cuda")
+    w = torch.randn((200, 256), generator=g, device="cuda")
+    ref = foam.block_linear(x, w)
+    torch.cuda.synchronize()
+    results = [None] * 4
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                results[i] = foam.block_linear(x, w)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(r, ref) for r in results)
+
+
+@pytest.mark.gpu
+def test_expanded_scales():
+    """One scale for all blocks, given as an expanded tensor."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    a, _ = operand(g, 150, 300, 1)
+    b, _ = operand(g, 300, 300, 1)
+    one = torch.full((1, 1), 0.25, device="cuda")
+    sa, sb = one.expand(150, 3), one.expand(3, 3)
+    ref, mag = product64(a, sa, b, sb)
+    check_product(foam.block_matmul(a, sa, b, sb, out_dtype=torch.float32), ref, mag, 300, torch.float32)
+    assert torch.equal(foam.dequantize_blocks(a, sa), a.float() * 0.25)
+
+
+@pytest.mark.gpu
 def test_codes_of_sites_through_a_layer():
     """Looked-up rows into an 8-bit layer, as a network over sites uses them:
     the gradient reaches the table through both."""
@@ -431,3 +490,27 @@ def test_entry_points_refuse_bad_arguments():
     wide = dict(lda=1280, ldb=1280, k=1280)
     assert matmul(ws=None, **wide) == 1 and matmul(size=need - 1, **wide) == 1 and "workspace" in message()
     assert matmul(m=0) == 0 and matmul(n=0) == 0
+
+    # the layer: m 300, n 256, k 128
+    saved = lib.sdfoam_block_linear_saved_bytes(300, 256, 128, 1, 1)
+    ws = lib.sdfoam_block_linear_workspace_bytes(300, 256, 128)
+    assert saved > 0 and ws > 0 and lib.sdfoam_block_linear_saved_bytes(300, 256, 128, 0, 0) == 0
+    assert lib.sdfoam_block_linear_workspace_bytes(1 << 31, 1, 1) == 0
+
+    def forward(x=p, xt=2, wt=0, n=256, y=p, sv=p, svb=saved, w=p, wsb=ws, bias=None, bt=0, ldx=128):
+        return lib.sdfoam_block_linear_forward(x, ldx, xt, 300, p, 128, wt, n, 128, bias, bt, y, sv, svb, 1, 1, w, wsb,
+                                               p, None)
+
+    assert forward(xt=3) == 2 and forward(wt=9) == 2 and forward(n=1 << 31) == 1
+    assert forward(svb=saved - 1) == 1 and forward(sv=None) == 1 and forward(wsb=0) == 1 and forward(w=None) == 1
+    assert "too small" in message()
+    assert forward(x=None) == 1 and forward(ldx=100) == 1 and forward(x=ctypes.c_void_p(4097)) == 1
+
+    def backward(dyt=2, kx=1, kw=1, sv=p, svb=saved, dx=p, dw=p, db=None, dbt=0, w=p, wsb=ws, dy=p):
+        return lib.sdfoam_block_linear_backward(dy, 256, dyt, 300, 256, 128, sv, svb, kx, kw, dx, 2, dw, 0, db, dbt, w,
+                                                wsb, p, None)
+
+    assert backward(kx=0) == 1 and backward(kw=0) == 1 and "kept" in message()
+    assert backward(dyt=3) == 2 and backward(svb=1) == 1 and backward(w=None) == 1
+    assert backward(dy=None) == 1 and backward(db=p, dbt=3) == 1
+    assert backward(dx=None, dw=None) == 0

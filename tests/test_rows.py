@@ -91,6 +91,11 @@ def test_lookup_shapes_and_strides():
         # an offset start: rows that no vector load may assume aligned
         flat = torch.randn(100 * 49 + 1, device="cuda")[1:].view(100, 49)
         assert torch.equal(foam.lookup_rows(flat, ids), flat[ids])
+    # site ids as a query returns them, not in the order of memory
+    sites = make_ids(ids[0], torch.uint32)
+    assert torch.equal(foam.lookup_rows(wide, sites.t()), wide[ids[0].t()])
+    with pytest.raises(RuntimeError, match="device of table"):
+        foam.lookup_rows(wide, ids.cpu())
     # nothing to look up, no columns, no rows
     assert foam.lookup_rows(wide, ids[:0]).shape == (0, 5, 6, 80)
     assert foam.lookup_rows(wide[:, :0], ids).shape == (4, 5, 6, 0)
