@@ -335,35 +335,44 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mask = P.bins - 1;
     const uint32_t tile0 = blockIdx.x * kSortTile, valid = min(kSortTile, P.n - tile0);
     const uint32_t first = warp * (32 * kSortItems) + lane;
-    uint32_t key[kSortItems], digit[kSortItems], rank[kSortItems];
+    // everything this block reads, before the ranking
+    uint32_t key[kSortItems], val[kSortItems], digit[kSortItems], rank[kSortItems];
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
         const uint32_t i = first + r * 32;
         key[r] = i < valid ? sort_key<I, FIRST>(P, tile0 + i) : 0u;
+        val[r] = FIRST ? tile0 + i : i < valid ? P.vals_in[tile0 + i] : 0u;
         digit[r] = i < valid ? (key[r] >> P.shift) & mask : 0xffffffffu;
+    }
+    constexpr int kBinsPer = kMaxBins / kSortThreads;
+    uint32_t total[kBinsPer], earlier[kBinsPer];
+#pragma unroll
+    for (int q = 0; q < kBinsPer; ++q) {
+        const int b = q * kSortThreads + int(threadIdx.x);
+        total[q] = earlier[q] = 0;
+        if (b < P.bins) {
+            if (FEW) {
+#pragma unroll 8
+                for (uint32_t t = 0; t < P.tiles; ++t) {
+                    const uint32_t x = P.counts[t * P.bins + b];
+                    total[q] += x;
+                    if (t < blockIdx.x) earlier[q] += x;
+                }
+            } else {
+                total[q] = P.totals[b];
+                earlier[q] = P.counts[size_t(b) * P.tiles + blockIdx.x];
+            }
+        }
     }
     rank_digits<kWarps, kSortItems>(digit, rank, u.counts, start, warp_sums, P.bins);
     // the digit's first place in the output: entries of smaller digits, this
     // digit's in earlier tiles, less the tile's own start
     __syncthreads();
     uint32_t carry = 0;
-    for (int b0 = 0; b0 < P.bins; b0 += kSortThreads) {
-        const int b = b0 + int(threadIdx.x);
-        uint32_t total = 0, earlier = 0;
-        if (b < P.bins) {
-            if (FEW) {
-#pragma unroll 8
-                for (uint32_t t = 0; t < P.tiles; ++t) {
-                    const uint32_t x = P.counts[t * P.bins + b];
-                    total += x;
-                    if (t < blockIdx.x) earlier += x;
-                }
-            } else {
-                total = P.totals[b];
-                earlier = P.counts[size_t(b) * P.tiles + blockIdx.x];
-            }
-        }
-        uint32_t incl = total;
+#pragma unroll
+    for (int q = 0; q < kBinsPer; ++q) {
+        const int b = q * kSortThreads + int(threadIdx.x);
+        uint32_t incl = total[q];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -377,7 +386,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
             if (uint32_t(w) < warp) before += warp_sums[w];
             all += warp_sums[w];
         }
-        if (b < P.bins) base[b] = before + incl - total + earlier - start[b];
+        if (b < P.bins) base[b] = before + incl - total[q] + earlier[q] - start[b];
         carry += all;
         __syncthreads();
     }
@@ -397,7 +406,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_digits_kernel(const Sort
 #pragma unroll
     for (int r = 0; r < kSortItems; ++r) {
         const uint32_t i = first + r * 32;
-        if (i < valid) u.vals[rank[r]] = FIRST ? tile0 + i : P.vals_in[tile0 + i];
+        if (i < valid) u.vals[rank[r]] = val[r];
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < valid; i += kSortThreads) {
