@@ -266,12 +266,12 @@ __device__ __forceinline__ uint32_t same_digit(uint32_t digit, bool valid, int w
     return peers;
 }
 
-// Ranks WARPS x ITEMS x 32 entries (warp w's are consecutive) by their digit
+// Ranks WARPS x items x 32 entries (warp w's are consecutive) by their digit
 // and puts them in order in shared memory: rank[] are this thread's places.
 // counts: [WARPS][bins], start: [bins + 1] first place of each digit.
 template <int WARPS, int ITEMS>
 __device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint32_t (&rank)[ITEMS], uint16_t *counts,
-                                            uint32_t *start, uint32_t *warp_sums, int bins) {
+                                            uint32_t *start, uint32_t *warp_sums, int bins, int items = ITEMS) {
     const int width = 31 - __clz(bins);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lt = (1u << lane) - 1u;
     constexpr uint32_t kThreads = WARPS * 32;
@@ -280,6 +280,7 @@ __device__ __forceinline__ void rank_digits(const uint32_t (&digit)[ITEMS], uint
     uint16_t *mine = counts + warp * bins;
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
+        if (r >= items) break;  // the same for every thread
         const uint32_t d = digit[r];
         const bool valid = d < uint32_t(bins);
         const uint32_t peers = same_digit(d, valid, width);
@@ -439,35 +440,37 @@ __global__ void __launch_bounds__(kBlockSortThreads) sort_block_kernel(const Sor
     uint32_t *keys = reinterpret_cast<uint32_t *>(raw), *vals = keys + kBlockSortThreads * kItems;
     uint16_t *counts = reinterpret_cast<uint16_t *>(vals + kBlockSortThreads * kItems);
     uint32_t *start = reinterpret_cast<uint32_t *>(counts + kWarps * kBlockSortBins), *warp_sums = start + kBlockSortBins;
-    const uint32_t first = (threadIdx.x >> 5) * (32 * kItems) + (threadIdx.x & 31);
+    // no more items per thread than there are: warp w's are consecutive
+    const int items = int((P.n + kBlockSortThreads - 1) / kBlockSortThreads);
+    const uint32_t first = (threadIdx.x >> 5) * (32 * items) + (threadIdx.x & 31);
     uint32_t key[kItems], val[kItems], digit[kItems], rank[kItems];
 #pragma unroll
     for (int r = 0; r < kItems; ++r) {
         val[r] = first + r * 32;
-        key[r] = val[r] < P.n ? sort_key<I, true>(P, val[r]) : 0u;
+        key[r] = r < items && val[r] < P.n ? sort_key<I, true>(P, val[r]) : 0u;
     }
     for (int shift = 0; shift < bits; shift += 8) {
 #pragma unroll
         for (int r = 0; r < kItems; ++r)
-            digit[r] = first + r * 32 < P.n ? (key[r] >> shift) & (kBlockSortBins - 1) : 0xffffffffu;
-        rank_digits<kWarps, kItems>(digit, rank, counts, start, warp_sums, kBlockSortBins);
+            digit[r] = r < items && first + r * 32 < P.n ? (key[r] >> shift) & (kBlockSortBins - 1) : 0xffffffffu;
+        rank_digits<kWarps, kItems>(digit, rank, counts, start, warp_sums, kBlockSortBins, items);
 #pragma unroll
         for (int r = 0; r < kItems; ++r)
-            if (first + r * 32 < P.n) {
+            if (r < items && first + r * 32 < P.n) {
                 keys[rank[r]] = key[r];
                 vals[rank[r]] = val[r];
             }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kItems; ++r)
-            if (first + r * 32 < P.n) {
+            if (r < items && first + r * 32 < P.n) {
                 key[r] = keys[first + r * 32];
                 val[r] = vals[first + r * 32];
             }
     }
 #pragma unroll
     for (int r = 0; r < kItems; ++r)
-        if (first + r * 32 < P.n) {
+        if (r < items && first + r * 32 < P.n) {
             P.keys_out[first + r * 32] = key[r];
             P.vals_out[first + r * 32] = val[r];
         }
