@@ -19,8 +19,7 @@
 //   * warps 4-11 read the accumulators back (warp w: TMEM lanes 32 (w % 4)
 //     .., half of the TN columns; one row per thread) and multiply-add them
 //     into registers while the tensor cores fill the next accumulator.  Their
-//     sums and two chunks of loads take the registers that the first four
-//     warps give up.
+//     sums take the registers that the first four warps give up.
 //
 // The operand with the rows on the TMEM lanes is P, the other Q.  Q is b
 // unless a has few rows (a single token to 64): then a's rows are the narrow
@@ -72,7 +71,7 @@ struct Shape {
     static constexpr int kCtas = PAIR ? 2 : 1;
     static constexpr uint32_t kQBytes = TN / kCtas * kBlockK;
     static constexpr uint32_t kStageBytes = kPBytes + kQBytes;  // per CTA
-    static constexpr int kStages = TN == 256 ? (PAIR ? 4 : 3) : TN == 128 ? 5 : TN == 64 ? 7 : 8;
+    static constexpr int kStages = TN == 256 ? 4 : TN == 128 ? 5 : TN == 64 ? 7 : 8;
     static constexpr int kAccs = TN == 256 ? 2 : 4;
     static constexpr uint32_t kTmemCols = uint32_t(TN) * kAccs;
     static constexpr int kGroups = 2, kCols = TN / kGroups;  // groups of four epilogue warps, their columns
@@ -316,9 +315,11 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) w[i] = w[i + 1];
         }
+        __syncwarp();
         asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
 #pragma unroll
         for (uint32_t turn = 0; turn < uint32_t(kGroups); ++turn) {
+            __syncwarp();
             if (turn > 0) asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
             if (group == turn) continue;
             if (odd) {
@@ -331,6 +332,7 @@ __device__ __forceinline__ void store_rows(const BlockParams &P, const CUtensorM
             for (int i = 1; i < kCols / 2; ++i) *reinterpret_cast<uint32_t *>(dst + 2 * i - odd) = w[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
         asm volatile("bar.sync %0, %1;" ::"r"(2 + quarter), "n"(32 * kGroups) : "memory");
         if (group == 0 && row0 < P.p_rows) {
             const uint32_t bytes = min(32u, P.p_rows - row0) * n * 2, whole = bytes & ~15u;
@@ -499,8 +501,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
     constexpr int kChunk = 8;
     // A scale per column is a value per column for every thread that holds one
     // row: at 128 bytes a cycle shared memory takes twice the MMAs' time to
-    // hand them out (4096^3: 111 us, 75 without those reads).  Where the tile is
-    // wide, a thread holds 4 rows of a quarter of the columns instead.
+    // hand them out (4096^3: 111 to 134 us in two runs, 75 to 89 without those
+    // reads).  Where the tile is wide, a thread holds 4 rows of a quarter of the
+    // columns instead (93 to 109).
     constexpr bool kPatch = QROWS && !SWAP && TN >= 128;
     constexpr uint32_t kPart = kTileP * TN / 4;  // float4 of a CTA's sums: [warp][columns / 4][lane]
     extern __shared__ unsigned char smem_raw[];
@@ -673,8 +676,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
             if (!SWAP && P.bias && P.splits == 1) {
                 // the sums start from the bias
                 if (t.tq != bias_tq) {
+                    __syncwarp();
                     asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
                     if (et < TN) bias_s[et] = t.tq * TN + et < P.q_rows ? bias_at(P, t.tq * TN + et) : 0.0f;
+                    __syncwarp();
                     asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
                     bias_tq = t.tq;
                 }
@@ -705,6 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                     one = QROWS ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * *q_sc;
                 }
                 if (!mbar_wait(acc_full + 8 * b, turn & 1, &abort_flag)) bad = true;
+                __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
                 if constexpr (kPatch) {

@@ -64,6 +64,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // bound (the clean-up waits).  The clock is read only after some polls: a
 // tile's wait is over by then.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+    if (mbar_try(bar, parity)) return true;
+    if (abort && *abort) return false;
     for (int i = 0; i < 64; ++i)
         if (mbar_try(bar, parity)) return true;
     const uint64_t t0 = global_ns();

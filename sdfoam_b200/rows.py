@@ -103,6 +103,8 @@ def lookup_rows(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> t
     adds to no gradient.  The product is fp32, rounded once."""
     if table.dim() != 2:
         raise RuntimeError("table must have 2 dimensions")
+    if table.shape[0] >= 2 ** 32:
+        raise RuntimeError("table must have fewer than 2^32 rows")
     _check("table", table, ids)
     if not (table.requires_grad and torch.is_grad_enabled()):
         return _lookup(table, ids, float(scale))

@@ -336,6 +336,24 @@ def test_calls_from_several_threads_and_streams():
 
 
 @pytest.mark.gpu
+def test_a_product_that_gave_up_is_reported():
+    """The word that a kernel writes when a wait runs out, written here by the
+    host: the next product and the check raise it once."""
+    from sdfoam_b200 import blocks
+    a, sa = foam.quantize_blocks(torch.randn((40, 128), device="cuda"))
+    ref = foam.block_matmul(a, sa, a, sa)
+    foam.check_block_flags()
+    word = blocks._flags[a.device.index][1]
+    for call in (lambda: foam.block_matmul(a, sa, a, sa), foam.check_block_flags):
+        torch.cuda.synchronize()
+        word[0] = 1
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            call()
+        assert torch.equal(foam.block_matmul(a, sa, a, sa), ref)
+        foam.check_block_flags()
+
+
+@pytest.mark.gpu
 def test_expanded_scales():
     """One scale for all blocks, given as an expanded tensor."""
     g = torch.Generator(device="cuda").manual_seed(8)

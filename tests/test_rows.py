@@ -241,6 +241,8 @@ def test_refusals():
         foam.lookup_rows(t, i.to(torch.int16))
     with pytest.raises(RuntimeError, match="columns"):
         foam.lookup_rows(torch.zeros((1, (1 << 20) + 1)), i)
+    with pytest.raises(RuntimeError, match="fewer than 2\\^32 rows"):
+        foam.lookup_rows(torch.zeros((1, 1)).expand(1 << 32, 1), i)
     with pytest.raises(RuntimeError, match="shape of ids"):
         foam.lookup_rows_backward(torch.zeros((4, 3)), i, 4)
     with pytest.raises(RuntimeError, match="num_rows"):
