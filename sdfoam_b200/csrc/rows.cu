@@ -156,8 +156,9 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 // the number of rows needs, of equal width).  A pass over tiles of 2048
 // counts the digits of each tile, scans the counts, and scatters: every warp
 // ranks its 256 consecutive entries by ballots over the digit's bits and its
-// own digit counts (__match_any_sync took 360 cycles a call here), the tile is put in order in shared memory and leaves in runs of
-// equal digits.  The first pass reads the ids themselves.
+// own digit counts (with __match_any_sync a pass over 2M entries takes 33 to
+// 38 us instead of 21), the tile is put in order in shared memory and leaves
+// in runs of equal digits.  The first pass reads the ids themselves.
 //
 // Launches count where there are few ids.  Up to 64 tiles need no scan: every
 // block adds up the counts of the tiles before its own, and a pass counts the
@@ -635,7 +636,6 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams P
 // a segment of few chunks itself; segments of many (hot ids) are shared by
 // the block's threads, each taking a contiguous run of the parts, and the
 // runs' sums are added in order.
-
 template <typename T, int VB>
 __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const SumParams P) {
     if (blockIdx.x >= P.join_blocks) {
