@@ -122,6 +122,8 @@ bool aligned_ids(const void *p, uint32_t id_type) {
     return (reinterpret_cast<uintptr_t>(p) & (id_type == SDFOAM_I64 ? 7u : 3u)) == 0;
 }
 
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // [R,4] attribute-typed rows: 16 bytes (float32) or 8 bytes (float16) each.
@@ -733,6 +735,8 @@ int sdfoam_block_quantize(const void *x, uint64_t ld, uint32_t dtype, uint64_t m
             return fail(SDFOAM_ERR_INVALID, "rows of values must be multiples of 16 bytes and 16-byte aligned");
         if (column_sums && (!turned || !workspace || sums_dtype > SDFOAM_BF16 || !aligned_to(column_sums, sums_dtype)))
             return fail(SDFOAM_ERR_INVALID, "column_sums need turned, a workspace and a type");
+        if ((values && !aligned4(scales)) || (turned && !aligned4(turned_scales)) || (column_sums && !aligned4(workspace)))
+            return fail(SDFOAM_ERR_INVALID, "scales and workspace must be 4-byte aligned");
     }
     if (m == 0 && k > 0 && column_sums) {
         cudaError_t z = cudaMemsetAsync(column_sums, 0, k * (sums_dtype == SDFOAM_F32 ? 4 : 2),
@@ -755,6 +759,7 @@ int sdfoam_block_dequantize(const void *values, uint64_t ldv, const float *scale
         return fail(SDFOAM_ERR_INVALID, "values, scales and out must be non-NULL");
     if (ldv < k || (ldv >> 40)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
     if (!aligned_to(out, dtype)) return fail(SDFOAM_ERR_INVALID, "out must be aligned to its elements");
+    if (!aligned4(scales)) return fail(SDFOAM_ERR_INVALID, "scales must be 4-byte aligned");
     cudaError_t e = launch_block_dequantize(values, ldv, scales, scale_row, scale_block, block_rows,
                                             static_cast<uint32_t>(m), static_cast<uint32_t>(k), dtype, out,
                                             reinterpret_cast<cudaStream_t>(stream));
@@ -783,6 +788,8 @@ int sdfoam_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint
         return fail(SDFOAM_ERR_INVALID, "a, b, their scales, out and error must be non-NULL");
     if (k > 0 && (lda % 16 || ldb % 16 || lda < k || ldb < k || (lda >> 40) || (ldb >> 40) || !aligned16(a) || !aligned16(b)))
         return fail(SDFOAM_ERR_INVALID, "rows of a and b must be multiples of 16 bytes and 16-byte aligned");
+    if (k > 0 && (!aligned4(a_scales) || !aligned4(b_scales) || !aligned4(error)))
+        return fail(SDFOAM_ERR_INVALID, "scales and error must be 4-byte aligned");
     if (ldo < n || (ldo >> 38)) return fail(SDFOAM_ERR_INVALID, "rows must be at least as far apart as their columns");
     if (!aligned_to(out, out_dtype) || (bias && !aligned_to(bias, bias_dtype)))
         return fail(SDFOAM_ERR_INVALID, "out and bias must be aligned to their elements");

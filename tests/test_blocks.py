@@ -532,3 +532,25 @@ def test_entry_points_refuse_bad_arguments():
     assert backward(dyt=3) == 2 and backward(svb=1) == 1 and backward(w=None) == 1
     assert backward(dy=None) == 1 and backward(db=p, dbt=3) == 1
     assert backward(dx=None, dw=None) == 0
+
+
+def test_entry_points_refuse_unaligned_scales():
+    """Scales, sums and the error word are read and written as 4-byte words."""
+    from sdfoam_b200 import build
+    build.build()
+    lib = _lib.load()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4098)
+
+    def quantize(s=p, ts=p, ws=p):
+        return lib.sdfoam_block_quantize(p, 32, 0, 4, 32, 1, p, 32, s, p, 16, ts, p, 0, ws, None)
+
+    def matmul(sa=p, sb=p, error=p):
+        return lib.sdfoam_block_matmul(p, 128, sa, 1, 1, 1, 300, p, 128, sb, 1, 1, 1, 256, 128, None, 0, p, 256, 2, p, 1 << 30,
+                                       error, None)
+
+    calls = [lambda: quantize(s=odd), lambda: quantize(ts=odd), lambda: quantize(ws=odd), lambda: matmul(sa=odd),
+             lambda: matmul(sb=odd), lambda: matmul(error=odd),
+             lambda: lib.sdfoam_block_dequantize(p, 32, odd, 1, 1, 1, 4, 32, 0, p, None)]
+    for call in calls:
+        assert call() == 1
+        assert "4-byte aligned" in lib.sdfoam_last_error().decode()
