@@ -211,10 +211,11 @@ def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, grad_mode):
         # x is kept (turned, in 8 bits) for the weight's gradient and the
-        # weight for x's
-        keep_w, keep_x = ctx.needs_input_grad[:2]
+        # weight for x's (needs_input_grad does not know the grad mode, which
+        # is off in here)
+        keep_w, keep_x = (grad_mode and need for need in ctx.needs_input_grad[:2])
         x, weight = _matrix(x), _matrix(weight)
         m, k = x.shape
         n = weight.shape[0]
@@ -243,7 +244,7 @@ class _BlockLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         (saved,) = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         m, n, k = ctx.sizes
         grad = _matrix(grad)
         dev = grad.device
@@ -259,7 +260,7 @@ class _BlockLinear(torch.autograd.Function):
                 saved.numel(), *ctx.kept, None if dx is None else dx.data_ptr(), _DTYPES[ctx.dtypes[0]],
                 None if dw is None else dw.data_ptr(), _DTYPES[ctx.dtypes[1]], None if db is None else db.data_ptr(),
                 0 if db is None else _DTYPES[db.dtype], ws.data_ptr(), nbytes, _flag(dev), _lib.stream(dev)))
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 def block_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -287,6 +288,6 @@ def block_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if bias is not None:
         _check_bias(bias, weight.shape[0], x.device)
     if x.dim() == 2:
-        return _BlockLinear.apply(x, weight, bias)
-    y = _BlockLinear.apply(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]), weight, bias)
+        return _BlockLinear.apply(x, weight, bias, torch.is_grad_enabled())
+    y = _BlockLinear.apply(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]), weight, bias, torch.is_grad_enabled())
     return y.reshape(*x.shape[:-1], weight.shape[0])

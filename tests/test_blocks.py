@@ -354,6 +354,35 @@ def test_a_product_that_gave_up_is_reported():
 
 
 @pytest.mark.gpu
+def test_inference_keeps_nothing(monkeypatch):
+    """Without gradients nothing is kept for a backward, whatever the weight
+    asks for; with them, what the inputs that ask need."""
+    lib = _lib.load()
+    inner, kept = lib.sdfoam_block_linear_forward, []
+
+    class Spy:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+
+        def sdfoam_block_linear_forward(self, *args):
+            kept.append(tuple(map(bool, args[14:16])))
+            return inner(*args)
+
+    monkeypatch.setattr(_lib, "load", Spy)
+    x = torch.randn((70, 200), device="cuda")
+    w = torch.randn((30, 200), device="cuda", requires_grad=True)
+    ref = foam.block_linear(x, w)
+    assert ref.requires_grad
+    with torch.no_grad():
+        y = foam.block_linear(x, w)
+    with torch.inference_mode():
+        z = foam.block_linear(x, w)
+    foam.block_linear(x.requires_grad_(), w.detach())
+    assert kept == [(True, False), (False, False), (False, False), (False, True)]
+    assert torch.equal(y, ref) and torch.equal(z, ref)
+
+
+@pytest.mark.gpu
 def test_expanded_scales():
     """One scale for all blocks, given as an expanded tensor."""
     g = torch.Generator(device="cuda").manual_seed(8)
