@@ -166,8 +166,9 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 // order).  180k ids with the scan and without it, the call: 47 and 42 us for
 // 41450 rows of 3 bf16, 137 and 125 us for 1M rows of 49 floats, 33 and 34 us
 // for 300 rows of 16; replayed in a graph 31 and 34, 117 and 116, 24 and 29.
-// 250k ids (123 tiles): the call 49 and 50, 148 and 143, 36 and 42.  Up to 8192 entries are sorted by one block in one launch (4097: the
-// same time on the GPU as five launches, 8 us less with the call).
+// 250k ids (123 tiles): the call 49 and 50, 148 and 143, 36 and 42.  Up to
+// 8192 entries are sorted by one block in one launch (4097: the same time on
+// the GPU as five launches, 8 us less with the call).
 
 constexpr int kSortThreads = 256;
 constexpr int kSortItems = 8;
