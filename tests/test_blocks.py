@@ -111,6 +111,33 @@ def test_quantize(dtype, block_rows, transpose):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_dequantize_rows(dtype, block_rows):
+    """Rows of any width, distance and start, scales of any order, and an
+    output that starts at any element, with a frame that stays as it was."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    lib = _lib.load()
+    for m, k in ((1, 1), (9000, 1), (3000, 3), (700, 5), (513, 8), (130, 217), (100, 124), (333, 132), (2, 20000), (300, 130)):
+        scales = torch.randn((m if block_rows == 1 else blocks(m), blocks(k)), generator=g, device="cuda")
+        for start, ld in ((0, -(-k // 16) * 16), (0, k + 5), (3, k + 16), (4, -(-k // 4) * 4 + 4), (8, -(-k // 8) * 8 + 8)):
+            store = torch.randint(0, 256, (start + m * ld,), generator=g, device="cuda").to(torch.uint8)
+            values = store.view(E4M3)[start:].view(m, ld)[:, :k]
+            # a product of 4 and 24 significant bits: exact in 64, rounded once
+            # to 32 and once to the output as the definition has it
+            ref = (values.double() * widen(scales, m, k)).float().to(dtype)
+            for s in (scales, scales.t().contiguous().t()):
+                assert torch.allclose(foam.dequantize_blocks(values, s, dtype), ref, rtol=0, atol=0, equal_nan=True)
+            frame = torch.full((m * k + 9,), 7, dtype=dtype, device="cuda")
+            torch.cuda.synchronize()
+            assert lib.sdfoam_block_dequantize(values.data_ptr(), ld, scales.data_ptr(), *scales.stride(), block_rows, m, k,
+                                               {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype],
+                                               frame[1:].data_ptr(), _lib.stream(frame.device)) == 0
+            assert torch.allclose(frame[1:1 + m * k].view(m, k), ref, rtol=0, atol=0, equal_nan=True)
+            assert frame[0] == 7 and (frame[1 + m * k:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_edges(block_rows):
     """Infinities, NaN, the smallest and largest numbers, ties, borders of the scale."""
     tiny = 2.0 ** -149
