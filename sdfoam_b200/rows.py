@@ -4,13 +4,14 @@ Site ids come out of this package as uint32 with UINT32_MAX for "none"
 (``nn``, ``farthest_neighbor``, the walk's ``depth_indices`` and site
 records), which torch cannot index with on a GPU.  ``lookup_rows`` takes them
 as they are: per-site attributes or learned codes at the sites of a query or
-a walk, differentiable with respect to the table.  The gradient is summed
-over the sorted ids in a fixed order, so a training step gives the same bits
-every run, where an index_add on the GPU does not.
+a walk, differentiable with respect to the table in reverse and forward mode.
+The gradient is summed over the sorted ids in a fixed order, so a training
+step gives the same bits every run, where an index_add on the GPU does not.
 """
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwad
 
 from . import _lib
 
@@ -67,9 +68,12 @@ def _lookup_backward(grad, ids, num_rows, scale):
 
 
 class _Lookup(torch.autograd.Function):
+    """Linear in table: the tangent of the rows is the lookup of the table's."""
+
     @staticmethod
     def forward(ctx, table, ids, scale):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.num_rows, ctx.scale = table.shape[0], scale
         return _lookup(table, ids, scale)
 
@@ -78,20 +82,35 @@ class _Lookup(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         return _LookupBackward.apply(grad, ids, ctx.num_rows, ctx.scale), None, None
 
+    @staticmethod
+    def jvp(ctx, table, ids, scale):
+        return lookup_rows(table, ctx.saved_tensors[0], ctx.scale)
+
 
 class _LookupBackward(torch.autograd.Function):
-    """Linear in grad, so its own gradient is the lookup again."""
+    """Linear in grad, so its own gradient is the lookup again, and its tangent
+    the gradient of grad's."""
 
     @staticmethod
     def forward(ctx, grad, ids, num_rows, scale):
         ctx.save_for_backward(ids)
-        ctx.scale = scale
+        ctx.save_for_forward(ids)
+        ctx.num_rows, ctx.scale = num_rows, scale
         return _lookup_backward(grad, ids, num_rows, scale)
 
     @staticmethod
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
         return _Lookup.apply(grad, ids, ctx.scale), None, None, None
+
+    @staticmethod
+    def jvp(ctx, grad, ids, num_rows, scale):
+        return lookup_rows_backward(grad, ctx.saved_tensors[0], ctx.num_rows, ctx.scale)
+
+
+def _differentiated(x: torch.Tensor) -> bool:
+    """Whether the result must carry a graph or a tangent."""
+    return (x.requires_grad and torch.is_grad_enabled()) or fwad.unpack_dual(x).tangent is not None
 
 
 def lookup_rows(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
@@ -106,7 +125,7 @@ def lookup_rows(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> t
     if table.shape[0] >= 2 ** 32:
         raise RuntimeError("table must have fewer than 2^32 rows")
     _check("table", table, ids)
-    if not (table.requires_grad and torch.is_grad_enabled()):
+    if not _differentiated(table):
         return _lookup(table, ids, float(scale))
     return _Lookup.apply(table, ids, float(scale))
 
@@ -123,6 +142,6 @@ def lookup_rows_backward(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, s
     if ids.numel() >= 2 ** 31:
         raise RuntimeError("the gradient takes fewer than 2^31 ids")
     _check("grad", grad, ids)
-    if not (grad.requires_grad and torch.is_grad_enabled()):
+    if not _differentiated(grad):
         return _lookup_backward(grad, ids, int(num_rows), float(scale))
     return _LookupBackward.apply(grad, ids, int(num_rows), float(scale))
