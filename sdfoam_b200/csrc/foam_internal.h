@@ -88,7 +88,7 @@ cudaError_t launch_radix_sort_pairs(uint32_t *const keys[2], uint32_t *const val
                                     uint32_t *totals, int &cur, cudaStream_t stream);
 
 // Table rows at given ids and the table's gradient (rows.cu).  dtype, itype:
-// SDFOAM_F32 / F16 / BF16, SDFOAM_I32 (also unsigned) / I64; ld in elements.
+// SDFOAM_F32 / F16 / BF16, SDFOAM_U32 / I32 / I64; ld in elements.
 size_t lookup_grad_workspace_bytes(uint32_t n, uint32_t rows, uint32_t columns);
 cudaError_t launch_lookup_rows(const void *table, uint32_t rows, uint32_t columns, size_t ld, uint32_t dtype,
                                const void *ids, uint64_t n, uint32_t itype, float scale, void *out,

@@ -39,11 +39,17 @@ namespace {
 // element and index types
 // --------------------------------------------------------------------------
 
+// The id as a row number below `limit`, or `none` when it names no such row.
 template <typename I>
-__device__ __forceinline__ uint32_t row_of(I id, uint32_t rows) {
-    // the id as a row number, or `rows` when it names none
-    if constexpr (sizeof(I) == 8) return static_cast<unsigned long long>(id) < rows ? uint32_t(id) : rows;
-    else return uint32_t(id) < rows ? uint32_t(id) : rows;
+__device__ __forceinline__ uint32_t row_of(I id, uint32_t limit, uint32_t none) {
+    if constexpr (sizeof(I) == 8) return static_cast<unsigned long long>(id) < limit ? uint32_t(id) : none;
+    else return uint32_t(id) < limit ? uint32_t(id) : none;
+}
+
+// The rows that ids of a type can name: 32-bit ids are compared as unsigned
+// numbers, where a negative signed one is 2^31 or more.
+uint32_t nameable_rows(uint32_t rows, uint32_t itype) {
+    return itype == SDFOAM_I32 ? std::min(rows, 1u << 31) : rows;
 }
 
 template <typename T>
@@ -121,7 +127,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const char *__re
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j) {
             col[j] = c;
-            row[j] = first + j * kLookupThreads + threadIdx.x < total ? row_of(*id, rows) : rows;
+            row[j] = first + j * kLookupThreads + threadIdx.x < total ? row_of(*id, rows, rows) : rows;
             c += step_col;
             id += step_row;
             if (c >= units) {
@@ -190,13 +196,14 @@ struct SortPass {
     uint32_t clear_counts;         // few tiles, first pass: words behind counts that later passes add to
     uint32_t *totals;              // [bins]
     uint32_t n, rows, tiles;
+    uint32_t named;                // rows that an id of the type can name; an id without a row sorts as `rows`
     int shift, bins;
     unsigned char *touched;        // cleared by the first pass
 };
 
 template <typename I, bool FIRST>
 __device__ __forceinline__ uint32_t sort_key(const SortPass &P, uint32_t i) {
-    if constexpr (FIRST) return row_of(static_cast<const I *>(P.ids)[i], P.rows);
+    if constexpr (FIRST) return row_of(static_cast<const I *>(P.ids)[i], P.named, P.rows);
     else return P.keys_in[i];
 }
 
@@ -805,7 +812,6 @@ cudaError_t lookup_unit(int vb, const void *table, uint32_t rows, size_t row_byt
 template <typename T>
 cudaError_t lookup_index(uint32_t itype, int vb, const void *table, uint32_t rows, size_t row_bytes, const void *ids,
                          uint64_t n, uint32_t columns, float scale, void *out, cudaStream_t stream) {
-    // 32-bit ids: a signed one below 0 is past every row as an unsigned one
     if (itype == SDFOAM_I64)
         return lookup_unit<T, long long>(vb, table, rows, row_bytes, ids, n, columns, scale, out, stream);
     return lookup_unit<T, uint32_t>(vb, table, rows, row_bytes, ids, n, columns, scale, out, stream);
@@ -909,6 +915,7 @@ cudaError_t launch_lookup_rows(const void *table, uint32_t rows, uint32_t column
     if (n == 0 || columns == 0) return cudaSuccess;
     const size_t bytes = size_t(columns) * type_size(dtype), row_bytes = ld * type_size(dtype);
     const int vb = std::min(unit_bytes(table, row_bytes, bytes), unit_bytes(out, bytes, bytes));
+    rows = nameable_rows(rows, itype);
     switch (dtype) {
         case SDFOAM_F32: return lookup_index<float>(itype, vb, table, rows, row_bytes, ids, n, columns, scale, out, stream);
         case SDFOAM_F16: return lookup_index<__half>(itype, vb, table, rows, row_bytes, ids, n, columns, scale, out, stream);
@@ -936,6 +943,7 @@ cudaError_t launch_lookup_rows_backward(const void *grad, size_t ld, uint32_t co
     S.totals = reinterpret_cast<uint32_t *>(ws + l.totals);
     S.n = n;
     S.rows = rows;
+    S.named = nameable_rows(rows, itype);
     S.touched = touched;
     int cur = 0;
     const cudaError_t e = itype == SDFOAM_I64 ? sort_ids<long long>(S, keys, vals, cur, stream)
