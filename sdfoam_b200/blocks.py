@@ -14,6 +14,7 @@ gradients are 8-bit products of operands quantized on the way.
 from __future__ import annotations
 
 import math
+import threading
 
 import torch
 
@@ -42,16 +43,20 @@ def _matrix(x: torch.Tensor) -> torch.Tensor:
 
 # One word per device in pinned host memory, which a kernel that gives up
 # waiting writes and the host reads without a copy: (tensor, its numpy view,
-# its address).
+# its address).  Made once, under the lock: kernels hold the address.
 _flags: dict = {}
+_flags_lock = threading.Lock()
 
 
 def _flag(device: torch.device) -> int:
     f = _flags.get(device.index)
     if f is None:
-        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-        f = _flags[device.index] = (t, t.numpy(), t.data_ptr())
-    elif f[1][0]:
+        with _flags_lock:
+            f = _flags.get(device.index)
+            if f is None:
+                t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                f = _flags[device.index] = (t, t.numpy(), t.data_ptr())
+    if f[1][0]:
         _raise(f)
     return f[2]
 
@@ -65,7 +70,7 @@ def check_block_flags():
     """Waits for the devices that have run 8-bit products and raises
     RuntimeError if one of them gave up waiting on the tensor-core pipeline
     (the next product on the device raises it too)."""
-    for index, f in _flags.items():
+    for index, f in list(_flags.items()):
         torch.cuda.synchronize(index)
         if f[1][0]:
             _raise(f)
