@@ -6,7 +6,7 @@
 // The inner sum runs on the tensor cores (tcgen05.mma kind::f8f6f4, fp32
 // accumulation in TMEM); the scales differ from block to block, so each
 // block's 128-wide product is read back from TMEM and added, times its scale,
-// to fp32 sums in registers.  A persistent CTA per SM walks units of (tile of
+// to fp32 sums in registers, whatever the scales' sizes (scale_factors).  A persistent CTA per SM walks units of (tile of
 // 128 x TN, slice of the reduction):
 //   * warp 0 (one lane) streams 128-byte wide tiles of both operands through
 //     a ring with TMA (128-byte swizzle; rows and columns past the ends read
@@ -42,6 +42,7 @@
 // Every wait is bounded: a CTA that gives up sets *error, writes NaN, waits
 // (bounded) for its own copies and MMAs and frees its TMEM.  No TMA multicast.
 #include <algorithm>
+#include <cfloat>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -235,6 +236,38 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+
+// A sum x of a block is 0 or from 2^-18 to 2^25 in size.  Its scaled value
+// x * p * q may be a number of fp32 (or zero) where a step on the way, p * q or
+// x * q, is not: there it is multiplied by two factors that share the exponent.
+
+// Whether p * q leaves fp32's normal numbers, with neither zero, infinite or NaN.
+__device__ __forceinline__ bool product_leaves(float p, float q) {
+    const float size = fabsf(__fmul_rn(p, q));
+    return !(size >= FLT_MIN && size <= FLT_MAX) && p != 0.0f && q != 0.0f && isfinite(p) && isfinite(q);
+}
+
+// False only where x * q stays within them for every such x: q from 2^-108 to 2^102.
+__device__ __forceinline__ bool scale_is_far(float q) {
+    return (__float_as_uint(q) & 0x7fffffffu) - __float_as_uint(0x1p-108f) > __float_as_uint(0x1p102f) - __float_as_uint(0x1p-108f);
+}
+
+// x * first * second, rounded after each step, for finite p and q.  A call:
+// inlined for each column it slows the loop beside it (4096^3 with a scale per
+// column: 112 to 117 us).
+__device__ __noinline__ float2 scale_factors(float p, float q) {
+    int i, j;
+    const float a = frexpf(p, &i), b = frexpf(q, &j);
+    const int e = i + j, first = max(-100, min(100, e));
+    return make_float2(ldexpf(__fmul_rn(a, b), first), ldexpf(1.0f, max(-149, min(127, e - first))));
+}
+
+// acc + x * q * p, the same bits as without the factors where they are not needed.
+__device__ __forceinline__ float add_scaled(float acc, float x, float p, float q) {
+    if (!scale_is_far(q) || !isfinite(p) || !isfinite(q)) return __fmaf_rn(__fmul_rn(x, q), p, acc);
+    const float2 f = scale_factors(p, q);
+    return __fmaf_rn(__fmul_rn(x, f.x), f.y, acc);
 }
 
 __device__ __forceinline__ float bias_at(const BlockParams &P, uint32_t n) {
@@ -668,6 +701,15 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
         unsigned char *row_stage = boxes + quarter * S::kGroups * S::kBoxBytes, *stage = row_stage + group * S::kBoxBytes;
         uint32_t done = 0, bias_tq = 0xffffffffu;
         bool bad = false;
+        // this warp has read an accumulator and its scales
+        auto release = [&](uint32_t b, uint32_t ss) {
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) {
+                arrive_at_first<PAIR>(acc_empty + 8 * b);
+                mbar_arrive(scale_empty + 8 * ss);
+            }
+        };
         for (uint32_t u = first_unit; u < P.units; u += unit_step) {
             const Unit t = unit_of(P, u);
             const uint32_t row0 = (t.tp * S::kCtas + rank) * kTileP + quarter * 32, row = row0 + lane;
@@ -683,82 +725,151 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
                     asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
                     bias_tq = t.tq;
                 }
+                const float *own = bias_s + group * kCols;
+                if constexpr (kPatch) {
 #pragma unroll
-                for (int i = 0; i < kCols / 2; ++i) {
-                    const int column = kPatch ? i / 4 * 8 + int(lane & 3u) * 2 : 2 * i;
-                    acc[i] = *reinterpret_cast<const uint64_t *>(bias_s + group * kCols + column);
+                    for (int i = 0; i < kCols / 2; ++i)
+                        acc[i] = *reinterpret_cast<const uint64_t *>(own + i / 4 * 8 + (lane & 3u) * 2);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kCols / 2; i += 2) {
+                        const float4 x = *reinterpret_cast<const float4 *>(own + 2 * i);
+                        acc[i] = pair(x.x, x.y);
+                        acc[i + 1] = pair(x.z, x.w);
+                    }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
             }
+            bool far = false;
             for (uint32_t kb = t.k0; kb < t.k1; ++kb, ++done) {
-                const uint32_t b = done % S::kAccs, turn = done / S::kAccs;
-                const uint32_t ss = done % S::kScaleStages;
-                if (!mbar_wait(scale_full + 8 * ss, (done / S::kScaleStages) & 1, &abort_flag)) bad = true;
-                const float *sc = scales + ss * S::kScaleFloats;
-                const float *q_sc = sc + kTileP + (QROWS ? group * kCols : group);
-                float one = 0.0f;
-                uint64_t p4[kPatch ? 4 : 1];
-                if constexpr (kPatch) {
+                for (; kb < t.k1; ++kb, ++done) {
+                    const uint32_t b = done % S::kAccs, turn = done / S::kAccs;
+                    const uint32_t ss = done % S::kScaleStages;
+                    if (!mbar_wait(scale_full + 8 * ss, (done / S::kScaleStages) & 1, &abort_flag)) bad = true;
+                    const float *sc = scales + ss * S::kScaleFloats;
+                    const float *q_sc = sc + kTileP + (QROWS ? group * kCols : group);
+                    if constexpr (QROWS) {
+                        // any of the warp's columns
+                        constexpr int kPer = kCols < 32 ? 1 : kCols / 32;
+                        struct alignas(4 * kPer) Piece { float q[kPer]; };
+                        const Piece piece = reinterpret_cast<const Piece *>(q_sc)[kCols < 32 ? lane % kCols : lane];
+                        far = false;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float p = sc[quarter * 32 + 8 * j + (lane >> 2)];
-                        p4[j] = pair(p, p);
+                        for (int i = 0; i < kPer; ++i) far |= scale_is_far(piece.q[i]);
                     }
-                } else {
-                    one = QROWS ? sc[quarter * 32 + lane] : sc[quarter * 32 + lane] * *q_sc;
-                }
-                if (!mbar_wait(acc_full + 8 * b, turn & 1, &abort_flag)) bad = true;
-                __syncwarp();
-                asm volatile("tcgen05.fence::after_thread_sync;");
-                const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
-                if constexpr (kPatch) {
+                    float one = 0.0f;
+                    uint64_t p4[kPatch ? 4 : 1];
+                    if constexpr (kPatch) {
 #pragma unroll
-                    for (int c = 0; c < kCols / 16; ++c) {
-                        const uint64_t *qp = reinterpret_cast<const uint64_t *>(q_sc + c * 16 + (lane & 3u) * 2);
-                        const uint64_t q2[2] = {qp[0], qp[4]};
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = sc[quarter * 32 + 8 * j + (lane >> 2)];
+                            p4[j] = pair(p, p);
+                        }
+                    } else {
+                        one = sc[quarter * 32 + lane];
+                        if constexpr (!QROWS) {
+                            // this row, which then adds nothing
+                            far = product_leaves(one, *q_sc);
+                            one = far ? 0.0f : one * *q_sc;
+                        }
+                    }
+                    if (!mbar_wait(acc_full + 8 * b, turn & 1, &abort_flag)) bad = true;
+                    __syncwarp();
+                    const bool some = __any_sync(0xffffffffu, far);
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    if (QROWS && some) break;
+                    const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
+                    if constexpr (kPatch) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t v[8];
-                            tmem_load_patch(v, addr + (uint32_t(16 * h) << 16) + c * 16);
+                        for (int c = 0; c < kCols / 16; ++c) {
+                            const uint64_t *qp = reinterpret_cast<const uint64_t *>(q_sc + c * 16 + (lane & 3u) * 2);
+                            const uint64_t q2[2] = {qp[0], qp[4]};
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t v[8];
+                                tmem_load_patch(v, addr + (uint32_t(16 * h) << 16) + c * 16);
+                                tmem_wait(v);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int g = i / 2, j = 2 * h + i % 2;
+                                    const uint64_t x = pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                                    fma_pair(acc[4 * (2 * c + g) + j], mul_pair(x, q2[g]), p4[j]);
+                                }
+                            }
+                        }
+                    } else {
+                        const uint64_t s2 = pair(one, one);
+#pragma unroll
+                        for (int c = 0; c < kCols / kChunk; ++c) {
+                            uint32_t v[kChunk];
+                            tmem_load(v, addr + c * kChunk);
                             tmem_wait(v);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int g = i / 2, j = 2 * h + i % 2;
-                                const uint64_t x = pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                                fma_pair(acc[4 * (2 * c + g) + j], x, mul_pair(p4[j], q2[g]));
+                            for (int i = 0; i < kChunk; i += 4) {
+                                uint64_t x = pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                                uint64_t y = pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                                if (QROWS) {
+                                    const float4 q = *reinterpret_cast<const float4 *>(q_sc + c * kChunk + i);
+                                    x = mul_pair(x, pair(q.x, q.y));
+                                    y = mul_pair(y, pair(q.z, q.w));
+                                }
+                                fma_pair(acc[(c * kChunk + i) / 2], x, s2);
+                                fma_pair(acc[(c * kChunk + i) / 2 + 1], y, s2);
                             }
                         }
                     }
+                    if (!QROWS && some) break;
+                    release(b, ss);
+                }
+                if (kb == t.k1) break;
+                // a block with scales that need the factors: with a scale per
+                // column the whole of it, element by element, else the rows
+                // that the loop above left out.  In that loop this code costs
+                // a tenth although it does not run (4096^3: 76 to 85 us; out
+                // here 74, and 112 with a scale per column, as without any
+                // check; 1M x 217 x 256 166 to 173)
+                const uint32_t b = done % S::kAccs, ss = done % S::kScaleStages;
+                const float *sc = scales + ss * S::kScaleFloats;
+                const uint32_t addr = tmem + ((quarter * 32) << 16) + b * TN + group * kCols;
+                if constexpr (QROWS) {
+                    const float *q_sc = sc + kTileP + group * kCols;
+#pragma unroll
+                    for (int i = 0; i < kCols / 8; ++i) {
+                        // as many loads as in the loop above
+                        const int c = kPatch ? i / 2 * 16 : i * 8, h = i % 2;
+                        uint32_t v[8];
+                        if constexpr (kPatch) tmem_load_patch(v, addr + (uint32_t(16 * h) << 16) + c);
+                        else tmem_load(v, addr + c);
+                        tmem_wait(v);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int g = e / 2, j = 2 * h + e % 2;
+                            const float p = sc[quarter * 32 + (kPatch ? 8 * j + (lane >> 2) : lane)];
+                            const float *q = q_sc + c + (kPatch ? 8 * g + (lane & 3u) * 2 : 2 * e);
+                            uint64_t &sum = acc[kPatch ? 4 * (c / 8 + g) + j : c / 2 + e];
+                            const float2 was = unpair(sum);
+                            sum = pair(add_scaled(was.x, __uint_as_float(v[2 * e]), p, q[0]),
+                                       add_scaled(was.y, __uint_as_float(v[2 * e + 1]), p, q[1]));
+                        }
+                    }
                 } else {
-                    const uint64_t s2 = pair(one, one);
+                    float2 f = make_float2(0.0f, 0.0f);
+                    if (far) f = scale_factors(sc[quarter * 32 + lane], sc[kTileP + group]);
 #pragma unroll
                     for (int c = 0; c < kCols / kChunk; ++c) {
                         uint32_t v[kChunk];
                         tmem_load(v, addr + c * kChunk);
                         tmem_wait(v);
 #pragma unroll
-                        for (int i = 0; i < kChunk; i += 4) {
+                        for (int i = 0; i < kChunk; i += 2) {
                             const uint64_t x = pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                            const uint64_t y = pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-                            uint64_t sx = s2, sy = s2;
-                            if (QROWS) {
-                                const float4 q = *reinterpret_cast<const float4 *>(q_sc + c * kChunk + i);
-                                sx = mul_pair(s2, pair(q.x, q.y));
-                                sy = mul_pair(s2, pair(q.z, q.w));
-                            }
-                            fma_pair(acc[(c * kChunk + i) / 2], x, sx);
-                            fma_pair(acc[(c * kChunk + i) / 2 + 1], y, sy);
+                            if (far) fma_pair(acc[(c * kChunk + i) / 2], mul_pair(x, pair(f.x, f.x)), pair(f.y, f.y));
                         }
                     }
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;");
-                __syncwarp();
-                if (lane == 0) {
-                    arrive_at_first<PAIR>(acc_empty + 8 * b);
-                    mbar_arrive(scale_empty + 8 * ss);
-                }
+                release(b, ss);
             }
             if (bad) {
 #pragma unroll
