@@ -1123,7 +1123,7 @@ cudaError_t launch_tiles(const CUtensorMap &mp, const CUtensorMap &mq, const CUt
         const unsigned warps = P.tiles_p * P.tiles_q * kEpiWarps;
         if (P.splits > 8)
             join_slices_kernel<TN, SWAP, true><<<warps * (S::kCols / join_columns<TN, true>()), kJoinThreads, 0, stream>>>(P);
-        else
+        else if constexpr (TN > 64)  // narrow tiles of so few slices are a cluster
             join_slices_kernel<TN, SWAP, false><<<warps, kJoinThreads, 0, stream>>>(P);
     }
     return cudaGetLastError();
@@ -1151,7 +1151,7 @@ cudaError_t launch_tn(const Plan &l, const CUtensorMap &mp, const CUtensorMap &m
 size_t block_matmul_workspace_bytes(uint32_t m, uint32_t n, uint32_t k) {
     if (m == 0 || n == 0 || k == 0) return 0;
     const Plan l = plan_of(m, n, k);
-    return l.splits > 1 && !l.cluster_join ? size_t(l.tiles_p) * l.tiles_q * l.splits * (l.pair ? 2 : 1) * kTileP * l.tn * 4 : 0;
+    return l.splits > 1 && !l.cluster_join ? size_t(l.tiles_p) * l.tiles_q * l.splits * kTileP * l.tn * 4 : 0;
 }
 
 cudaError_t launch_block_matmul(const void *a, uint64_t lda, const float *a_scales, uint64_t a_scale_row,
