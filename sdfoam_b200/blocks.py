@@ -37,7 +37,11 @@ def _cuda(what: str, x: torch.Tensor, device=None):
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
-    """x itself when its rows are contiguous (any distance apart), else a copy."""
+    """x itself when its rows are contiguous (any distance apart), else a copy.
+    A view that negates as it is read (the imaginary part of a conjugate) is
+    written out: the kernels read memory."""
+    if x.is_neg():
+        x = x.resolve_neg()
     return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
 
 
@@ -197,7 +201,7 @@ def block_matmul(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
             _cuda(what, t, dev)
     if bias is not None:
         _check_bias(bias, n, dev)
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     lib = _lib.load()
     nbytes = lib.sdfoam_block_matmul_workspace_bytes(m, n, k)
     with _lib.on(dev):
@@ -232,7 +236,7 @@ class _BlockLinear(torch.autograd.Function):
         nbytes = lib.sdfoam_block_linear_workspace_bytes(m, n, k)
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         if bias is not None:
-            bias = bias.contiguous()
+            bias = bias.resolve_neg().contiguous()
         with _lib.on(dev):
             _lib.check(lib.sdfoam_block_linear_forward(
                 x.data_ptr(), max(x.stride(0), k), _DTYPES[x.dtype], m, weight.data_ptr(), max(weight.stride(0), k),

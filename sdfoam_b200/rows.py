@@ -34,7 +34,11 @@ def _check(what: str, rows: torch.Tensor, ids: torch.Tensor):
 
 
 def _matrix(x: torch.Tensor) -> torch.Tensor:
-    """x itself when its rows are contiguous (any distance apart), else a copy."""
+    """x itself when its rows are contiguous (any distance apart), else a copy.
+    A view that negates as it is read (the imaginary part of a conjugate) is
+    written out: the kernels read memory."""
+    if x.is_neg():
+        x = x.resolve_neg()
     ld = x.stride(0)
     return x if x.stride(1) == 1 and ld >= x.shape[1] else x.contiguous()
 
