@@ -506,8 +506,10 @@ SDFOAM_API int sdfoam_block_dequantize(const void *values, uint64_t ldv, const f
  *   out[m, n] = sum_j a_scales[m, j] b_scales[n, j] sum_(k in block j) a[m, k] b[n, k] + bias[n]
  * a [m, k] and b [n, k] e4m3, lda and ldb bytes between rows (multiples of 16,
  * 16-byte aligned); scales any fp32 values, one per block_rows (1 or 128) rows
- * and 128 columns, addressed as in sdfoam_block_dequantize.  Sums are fp32 in a fixed order; bias
- * (NULL: none) of bias_dtype; out of out_dtype with ldo elements between rows.
+ * and 128 columns, addressed as in sdfoam_block_dequantize (the product of two
+ * scales may leave fp32 where the sum times both does not).  Sums are fp32 in a
+ * fixed order; bias (NULL: none) of bias_dtype; out of out_dtype with ldo
+ * elements between rows.
  * *error (device-accessible int) is set to 1 if a tile gave up waiting for its
  * copies or MMAs (its outputs are NaN).  Workspace:
  * sdfoam_block_matmul_workspace_bytes (0: none), 16-byte aligned. */
@@ -567,7 +569,9 @@ SDFOAM_API int sdfoam_trace_forward_noalloc(const sdfoam_foam *foam,
 /* Message of the last failing call on this thread ("" if none). */
 SDFOAM_API const char *sdfoam_last_error(void);
 
-/* ABI version of this header. */
+/* ABI version of this header: 5.  The entry points of table rows and 8-bit
+ * products were added to it without a new number; a host that may meet an older
+ * library looks for their symbols. */
 SDFOAM_API int sdfoam_abi_version(void);
 
 #ifdef __cplusplus

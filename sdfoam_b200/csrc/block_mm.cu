@@ -30,14 +30,15 @@
 // them through its shared memory, otherwise they go to the workspace and a
 // second launch adds them.
 //
-// What bounds it.  Small reductions (sites x 256): HBM -- 1M x 256 x 256 in
-// 138 us, 5.9 TB/s, 1M x 217 x 256 in 161.  Large products: the pass over the
-// accumulators between two blocks.  8192^3 takes 399 us when the tensor cores
-// add up the whole reduction (2750 TFLOP/s, at the power limit), 427 with an
-// accumulator per block that nobody reads, and 510 with the scaled sums (2150);
+// What bounds it.  Small reductions (sites x 256): HBM -- 1048576 x 256 x 256
+// in 135 us, 6.0 TB/s, 1048577 x 217 x 256 with a bias in 173 (162 without).
+// Large products: the pass over the accumulators between two blocks.  In short
+// runs 8192^3 takes 399 us when the tensor cores add up the whole reduction
+// (2750 TFLOP/s), 427 with an accumulator per block that nobody reads, and 510
+// with the scaled sums (2150); back to back, at the power limit, 589 (1870).
 // TMEM holds two accumulators of a 256-column tile, so the MMAs of a block
 // wait for the reads of the block before last.  A CTA pair halves the operand
-// bytes per SM (one CTA per tile: 565 us).
+// bytes per SM (one CTA per tile, short runs: 565 us).  No kernel spills.
 //
 // Every wait is bounded: a CTA that gives up sets *error, writes NaN, waits
 // (bounded) for its own copies and MMAs and frees its TMEM.  No TMA multicast.
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_mm_kernel(const __grid_cons
     // row: at 128 bytes a cycle shared memory takes twice the MMAs' time to
     // hand them out (4096^3: 111 to 134 us in two runs, 75 to 89 without those
     // reads).  Where the tile is wide, a thread holds 4 rows of a quarter of the
-    // columns instead (93 to 109).
+    // columns instead (93 to 112; 74 with a scale per 128 columns).
     constexpr bool kPatch = QROWS && !SWAP && TN >= 128;
     constexpr uint32_t kPart = kTileP * TN / 4;  // float4 of a CTA's sums: [warp][columns / 4][lane]
     extern __shared__ unsigned char smem_raw[];

@@ -15,9 +15,11 @@
 // along that axis.  One pass over 128 x 128 tiles in registers writes either
 // or both, so the input is read once.  Scales are stored block by block, the
 // rows of one block of columns next to each other, as a product's tile reads
-// them.  HBM bounds it (2 or 4 bytes in, one
-// or two out per element): 1M x 256 bf16 turned in 138 us, 5.8 TB/s; 276 when
-// each tile waited for its own loads.
+// them.  HBM bounds it (2 or 4 bytes in, one or two out per element):
+// 1048576 x 256 bf16 turned in 141 us, 5.7 TB/s, in rows in 133, fp32 237 and
+// 199 (turned 276 when each tile waited for its own loads).  Rows that are not
+// whole 16-byte pieces are read element by element: 1048576 x 217 bf16 244 us
+// in rows, fp32 273.
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -330,10 +332,11 @@ __global__ void __launch_bounds__(1024) add_sums_kernel(const float *__restrict_
 // 16 bytes of out per thread and turn.  Where rows of values are as aligned
 // (ALIGNED), a turn is one load of values and one of a scale, all turns' loads
 // before the first store; elsewhere a byte per element, and a scale where a
-// block or a row begins.  1M x 256 turned into fp32 195 us, in rows into bf16
-// 116: 6.6 TB/s, HBM (2 turns 221 and 129; 4 bytes of values to a turn, each
-// turn waiting for its loads, 247 and 216).  1M x 217 into bf16 302, bound by
-// the byte loads (544 with one element and one division per turn).
+// block or a row begins.  1048576 x 256 turned into fp32 201 us, 6.7 TB/s, in
+// rows into bf16 126: HBM (1000000 x 256: 195 and 116; 2 turns 221 and 129; 4
+// bytes of values to a turn, each turn waiting for its loads, 247 and 216).
+// 1048576 x 217 into bf16 316, bound by the byte loads (1000000 rows: 302, and
+// 544 with one element and one division per turn).
 template <typename T>
 __device__ __forceinline__ void store16(T *p, const float *v);
 template <>

@@ -23,7 +23,8 @@
 // (312 MB at least; 425 move, since 196-byte rows start anywhere in a 64-byte
 // line); the gradient of 2M rows of 48 floats in 190 us, of which the sums
 // take 104 (5.4 TB/s), the sort 68 and the joins 17; of 512k bf16 rows of 256
-// into 1M in 193 (sums 86, zeros and joins 65, sort 42).
+// into 1M in 193 (sums 86, zeros and joins 65, sort 42).  The lookups of 16-bit
+// elements by 16 bytes, 8 units a thread, spill 4 bytes; no other kernel does.
 #include <algorithm>
 
 #include <cuda_bf16.h>

@@ -28,8 +28,10 @@ Other shapes and the CPU use the plain PyTorch layers below.
 
 `dtype=torch.float8_e4m3fn` keeps float32 weights and bf16 activations and
 runs every linear layer as an 8-bit product (blocks.block_linear: e4m3 with a
-scale per block of 128, forward and both gradients), for networks wide enough
-that the products' rate counts; any width and depth, CUDA only.
+scale per block of 128, forward and both gradients); any width and depth, CUDA
+only, no eikonal term.  Forward and backward of 65536 points: 1024 wide 6.4 ms,
+the bf16 layers 8.6; 256 wide 3.0, the fused bf16 path 3.2; of 1048576 points
+256 wide 16.6 against 8.7, where the fused path's softplus in the layer counts.
 """
 from __future__ import annotations
 
